@@ -138,6 +138,124 @@ int spinn_cuda_conv2d_noalloc(const float *x, const float *w, const float *bias,
                               int stride_h, int stride_w, int pad_h, int pad_w, int fused_act,
                               void *stream);
 
+/* ------------------------------------------------------------------ decoder serving operators */
+
+/* Operators of a decoding step on device memory, queued on the caller's stream: a paged key-value
+ * cache with its append, its attention of one new token per sequence and its eviction by
+ * accumulated attention weight.  The reference has no counterpart.
+ *
+ * Every pointer is device memory of the current device.  `stream` (NULL = the legacy default
+ * stream) must belong to the current device; nothing is waited for and nothing is allocated, so
+ * calls may be captured into CUDA graphs.  A call that needs a workspace takes it from the
+ * caller (the _workspace function gives its size, 16-byte aligned, contents irrelevant before
+ * and after); two calls that may overlap on the GPU need two workspaces.  Arguments are checked
+ * before any work is queued (SPINN_CUDA_EINVAL).  What only the device can see -- a page number
+ * outside the pool, a length beyond the table -- is skipped by the kernel without touching
+ * memory, and reported by the next spinn_cuda_stream_sync. */
+
+/* Element types: ENNF / ONNX codes. */
+#define SPINN_CUDA_FP32 1
+#define SPINN_CUDA_FP16 10
+#define SPINN_CUDA_BF16 16
+
+/* Waits for `stream` and returns (and clears) the deferred error of the operators below on the
+ * current device: SPINN_CUDA_EINVAL for a bad page or length, SPINN_CUDA_ETIMEOUT for an
+ * expired wait.  Not during capture. */
+int spinn_cuda_stream_sync(void *stream);
+
+/* Two page pools of one shape: keys and values, [num_pages][page_size][kv_heads][head_dim] with
+ * any strides (elements) and contiguous head_dim <= 256. */
+typedef struct {
+    void *k, *v;
+    int64_t page_stride, token_stride, head_stride;
+    int32_t dtype; /* SPINN_CUDA_FP32 / _FP16 / _BF16 */
+    int32_t num_pages, page_size, kv_heads, head_dim;
+    int32_t reserved; /* 0 */
+} SpinnCudaCache;
+
+/* Which pages hold each sequence: row s lists the pages of tokens 0 .. page_size - 1,
+ * page_size .. 2 page_size - 1, ... of sequence s; entries past its length are never read.
+ * lens[s] tokens of sequence s are in the cache. */
+typedef struct {
+    const int32_t *pages;
+    const int32_t *lens;
+    int64_t row_stride;
+    int32_t seqs, max_pages;
+} SpinnCudaPageTable;
+
+/* Appends new tokens: rows [starts[s], starts[s + 1]) of k and v ([tokens][kv_heads][head_dim],
+ * strides in elements, the cache's type) become tokens lens[s], lens[s] + 1, ... of sequence s.
+ * starts == NULL: one new token for each sequence (tokens == seqs).  lens is not changed.  Two
+ * sequences may not write to the same page. */
+typedef struct {
+    const void *k, *v;
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    const int32_t *starts;
+    int32_t tokens;
+    int32_t reserved; /* 0 */
+} SpinnCudaAppend;
+int spinn_cuda_cache_append(const SpinnCudaCache *cache, const SpinnCudaPageTable *table,
+                            const SpinnCudaAppend *rows, void *stream);
+
+/* Attention of one new token per sequence over its cached tokens:
+ *   y[s][h] = sum_t p[s][h][t] v[s][h / group][t],  p = softmax over t < lens[s] of
+ *   scale * q[s][h] . k[s][h / group][t],  group = q_heads / kv_heads.
+ * q and y are [seqs][q_heads][head_dim] of the cache's type (strides in elements).  A sequence
+ * of length 0 gets zeros.  Sums and probabilities are held in fp32 and y is rounded once.
+ * weights_out, when not NULL ([seqs][kv_heads][>= lens[s]] fp32, group <= 16, weights_capacity
+ * entries per row): weights_out[s][j][t] = weights_in[s][j][t] + the sum of p[s][h][t] over the
+ * heads h of group j, for t < lens[s]; entries beyond are left as they were.  weights_in NULL
+ * counts as zeros; it may be weights_out itself. */
+typedef struct {
+    const void *q;
+    void *y;
+    int64_t q_seq_stride, q_head_stride, y_seq_stride, y_head_stride;
+    const float *weights_in;
+    float *weights_out;
+    int64_t win_seq_stride, win_head_stride, wout_seq_stride, wout_head_stride;
+    int32_t weights_capacity;
+    int32_t q_heads;
+    float scale;
+    int32_t reserved; /* 0 */
+} SpinnCudaAttention;
+size_t spinn_cuda_paged_attention_workspace(const SpinnCudaCache *cache, const SpinnCudaPageTable *table,
+                                            const SpinnCudaAttention *a);
+int spinn_cuda_paged_attention(const SpinnCudaCache *cache, const SpinnCudaPageTable *table,
+                               const SpinnCudaAttention *a, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Cuts every sequence back to n = min(lens[s], budget) tokens, for each head by itself.  Kept are
+ * the last r = min(recent, n) tokens and, of the others, the n - r with the largest accumulated
+ * weight (equal weights: the earlier token; NaN counts as the lowest), in their order: kept[s][j]
+ * lists their slots (budget entries, -1 past n), their rows move to tokens 0 .. n - 1 of the
+ * pages in `out`, weights_out[s][j][0 .. n) are their weights and [n, lens[s]) becomes 0 (entries
+ * beyond are left as they were).  new_lens[s] = n.
+ * out_pages == the table's pages (the same pointer): in place; then no page may belong to two
+ * sequences, and out_row_stride is the table's.  Otherwise out_pages names pages that no
+ * sequence of the call reads, enough for n tokens per row.  weights_out may be weights_in. */
+typedef struct {
+    const float *weights_in;
+    float *weights_out;
+    int64_t win_seq_stride, win_head_stride, wout_seq_stride, wout_head_stride;
+    const int32_t *out_pages;
+    int64_t out_row_stride;
+    int32_t out_max_pages;
+    int32_t weights_capacity;
+    int32_t *new_lens;
+    int32_t *kept; /* [seqs][kv_heads][budget], contiguous */
+    int32_t budget, recent;
+} SpinnCudaEvict;
+int spinn_cuda_cache_evict(const SpinnCudaCache *cache, const SpinnCudaPageTable *table, const SpinnCudaEvict *e,
+                           void *stream);
+
+/* Diagnostics (host only): element offset of token `pos` of a table row of max_pages entries in a
+ * contiguous pool, or a negative value when its page is outside the pool or pos outside the
+ * row. */
+int64_t spinn_cuda_diag_cache_slot(const int32_t *row, int max_pages, int pos, int page_size, int num_pages,
+                                   int64_t page_stride, int64_t token_stride);
+/* Diagnostics (host only): attention's split of `units` tiles over `workers`: out3 = {first unit
+ * of `worker`, its end, the worker that owns `unit`}. */
+int spinn_cuda_diag_attention_share(int64_t units, int workers, int worker, int64_t unit, int64_t *out3);
+
 /* ------------------------------------------------------------------ model level */
 
 typedef struct SpinnCudaModel SpinnCudaModel;

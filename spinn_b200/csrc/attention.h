@@ -1,0 +1,57 @@
+// attention.h -- parameters of the paged attention launch (attention.cuh), and the instantiations
+// for each cache type, one translation unit each.
+#pragma once
+#include "cache.h"
+
+namespace spinn {
+
+// What a worker leaves for the join: its first segment when an earlier worker began it (kind 0),
+// and its last one when a later worker ends it (kind 1).  A segment is one (sequence, head
+// block); it begins at unit `begin`, w0 / w1 are its first and last worker, and [lo, hi) are this
+// worker's own units of it.
+struct Piece {
+  int s, hb;  // s < 0: none
+  int w0, w1;
+  long long begin, lo, hi;
+};
+
+struct AttnParams {
+  CacheView c;
+  const void* q;
+  void* y;
+  long long q_seq, q_head, y_seq, y_head;
+  int q_heads, group, gblocks, hblocks;  // hblocks = kv_heads * gblocks
+  int capacity;                          // longest allowed length
+  bool vec;                              // 16-byte loads of the cache
+  float scale_log2;
+  const float* win;
+  float* wout;
+  long long win_seq, win_head, wout_seq, wout_head;
+  float* part;    // [worker][2][NR * 32] unnormalised outputs, in register order
+  float* ml;      // [worker][2][2][GB] maxima and sums
+  Piece* pieces;  // [worker][2]
+  float* logits;  // [unit][TK][GB], scores in log2 units (weights only)
+};
+
+// CTAs of a launch and the bytes of each part of its workspace.
+struct AttnPlan {
+  int workers;
+  size_t part, ml, pieces, logits;
+};
+
+inline size_t up256(size_t b) { return (b + 255) & ~size_t(255); }
+
+// Heads of one block: a wider group is split into blocks that each read the cache.
+inline int attention_head_block(int bytes, int group) {
+  const int small = bytes == 2 ? 8 : 1, large = bytes == 2 ? 16 : 8;
+  return group <= small ? small : large;
+}
+
+AttnPlan attention_plan_fp16(const AttnParams& p, int sms, bool weights);
+AttnPlan attention_plan_bf16(const AttnParams& p, int sms, bool weights);
+AttnPlan attention_plan_fp32(const AttnParams& p, int sms, bool weights);
+int attention_launch_fp16(const AttnParams& p, const AttnPlan& pl, cudaStream_t st);
+int attention_launch_bf16(const AttnParams& p, const AttnPlan& pl, cudaStream_t st);
+int attention_launch_fp32(const AttnParams& p, const AttnPlan& pl, cudaStream_t st);
+
+}  // namespace spinn

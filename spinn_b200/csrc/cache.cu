@@ -1,0 +1,621 @@
+// cache.cu -- the paged key-value cache: host checks shared by its entry points, appending new
+// tokens, and eviction by accumulated attention weight.  Attention itself is in attention.cu.
+#include <algorithm>
+#include <map>
+#include <mutex>
+
+#include "cache.h"
+#include "internal.h"
+#include "launch.h"
+#include "ptx.cuh"
+
+namespace spinn {
+
+// One word per device, in the library's own image: no allocation, so that a first call may be a
+// captured one.
+__device__ unsigned g_decode_err = 0;
+
+int decode_error_word(int device, unsigned** word) {
+  static std::mutex mu;
+  static std::map<int, unsigned*> addr;
+  std::lock_guard<std::mutex> lk(mu);
+  unsigned*& a = addr[device];
+  if (!a) {
+    void* p = nullptr;
+    SPINN_CUDA_TRY(cudaGetSymbolAddress(&p, g_decode_err));
+    a = static_cast<unsigned*>(p);
+  }
+  *word = a;
+  return 0;
+}
+
+int dtype_bytes(int dtype) {
+  return dtype == SPINN_CUDA_FP32 ? 4 : (dtype == SPINN_CUDA_FP16 || dtype == SPINN_CUDA_BF16) ? 2 : 0;
+}
+
+int check_stream_device(const char* who, void* stream, int* device) {
+  SPINN_CUDA_TRY(cudaGetDevice(device));
+  if (stream) {
+    // a capturing stream may not be asked; a launch into one of another device fails by itself
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    SPINN_CUDA_TRY(cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &cap));
+    if (cap != cudaStreamCaptureStatusNone) return 0;
+    int sdev = -1;
+    SPINN_CUDA_TRY(cudaStreamGetDevice(static_cast<cudaStream_t>(stream), &sdev));
+    SPINN_CHECK_ARG(sdev == *device, "%s: stream belongs to device %d, the current device is %d", who, sdev, *device);
+  }
+  return 0;
+}
+
+int cache_view(const char* who, const SpinnCudaCache* c, const SpinnCudaPageTable* t, CacheView* v) {
+  SPINN_CHECK_ARG(c && t, "%s: cache and page table are required", who);
+  SPINN_CHECK_ARG(c->k && c->v && t->pages && t->lens, "%s: null pool, page table or lengths", who);
+  SPINN_CHECK_ARG(dtype_bytes(c->dtype), "%s: element type %d not supported (fp32, fp16 or bf16)", who, c->dtype);
+  SPINN_CHECK_ARG(c->num_pages > 0 && c->page_size > 0 && c->kv_heads > 0 && c->kv_heads <= 65535,
+                  "%s: bad pool geometry (%d pages of %d tokens, %d heads)", who, c->num_pages, c->page_size,
+                  c->kv_heads);
+  SPINN_CHECK_ARG(c->head_dim > 0 && c->head_dim <= 256, "%s: head_dim %d outside [1, 256]", who, c->head_dim);
+  SPINN_CHECK_ARG(c->page_stride >= 0 && c->token_stride >= 0 && c->head_stride >= 0, "%s: negative stride", who);
+  SPINN_CHECK_ARG(t->seqs > 0 && t->max_pages > 0 && t->row_stride >= 0, "%s: bad page table (%d rows of %d)", who,
+                  t->seqs, t->max_pages);
+  v->k = c->k;
+  v->v = c->v;
+  v->page_stride = c->page_stride;
+  v->token_stride = c->token_stride;
+  v->head_stride = c->head_stride;
+  v->num_pages = c->num_pages;
+  v->page_size = c->page_size;
+  v->kv_heads = c->kv_heads;
+  v->dim = c->head_dim;
+  v->table = t->pages;
+  v->table_stride = t->row_stride;
+  v->max_pages = t->max_pages;
+  v->seqs = t->seqs;
+  v->lens = t->lens;
+  const int es = dtype_bytes(c->dtype);
+  SPINN_CHECK_ARG(((uintptr_t)v->k | (uintptr_t)v->v) % es == 0 &&
+                      ((uintptr_t)v->table | (uintptr_t)v->lens) % 4 == 0,
+                  "%s: misaligned pointer", who);
+  return 0;
+}
+
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+bool cache_vec16(const CacheView& v, int bytes) {
+  const int per = 16 / bytes;
+  return aligned16(v.k) && aligned16(v.v) && v.dim % per == 0 && v.page_stride % per == 0 &&
+         v.token_stride % per == 0 && v.head_stride % per == 0;
+}
+
+namespace {
+
+// ------------------------------------------------------------------ append
+struct AppendParams {
+  CacheView c;
+  const void* k;
+  const void* v;
+  long long k_tok, k_head, v_tok, v_head;
+  const int* starts;
+  int tokens;
+};
+
+// One warp copies one token's key rows or value rows (every head): U is the copied unit, a
+// 16-byte vector where pointers, strides and head_dim allow it, one element otherwise.  Bound by
+// launch latency for a decoding step and by HBM for prompts; four independent loads per lane are
+// in flight.
+template <typename U, int ESZ>
+__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
+  const int lane = threadIdx.x & 31;
+  const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int tok = (int)(unit >> 1);
+  const bool is_v = unit & 1;
+  if (tok >= p.tokens) return;
+  int seq = tok, first = tok;
+  if (p.starts) {
+    // the last sequence whose first row is at or before tok (empty sequences share their start)
+    int lo = 0, hi = p.c.seqs;  // starts[lo] <= tok < starts[hi]
+    if (p.starts[0] > tok || p.starts[hi] <= tok) {
+      if (lane == 0) atomicOr(p.c.err, kCacheBadLength);
+      return;
+    }
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (p.starts[mid] <= tok)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    seq = lo;
+    first = p.starts[lo];
+  }
+  const long long pos = (long long)p.c.lens[seq] + (tok - first);
+  if (p.c.lens[seq] < 0 || pos >= cache_capacity(p.c.max_pages, p.c.page_size)) {
+    if (lane == 0) atomicOr(p.c.err, kCacheBadLength);
+    return;
+  }
+  const long long slot = cache_slot(p.c.table + seq * p.c.table_stride, (int)pos, p.c.page_size, p.c.num_pages,
+                                    p.c.page_stride, p.c.token_stride);
+  if (slot < 0) {
+    if (lane == 0) atomicOr(p.c.err, kCacheBadPage);
+    return;
+  }
+  constexpr int PER = sizeof(U) / ESZ;
+  const int row = p.c.dim / PER, total = row * p.c.kv_heads;
+  const long long src_tok = is_v ? p.v_tok : p.k_tok, src_head = is_v ? p.v_head : p.k_head;
+  const U* src = reinterpret_cast<const U*>(static_cast<const char*>(is_v ? p.v : p.k) + tok * src_tok * ESZ);
+  U* dst = reinterpret_cast<U*>(static_cast<char*>(is_v ? p.c.v : p.c.k) + slot * ESZ);
+  const long long sh = src_head / PER, dh = p.c.head_stride / PER;
+  for (int i0 = lane; i0 < total; i0 += 128) {
+    U r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + 32 * j;
+      if (i < total) {
+        const int h = i / row;
+        r[j] = src[h * sh + (i - h * row)];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + 32 * j;
+      if (i < total) {
+        const int h = i / row;
+        dst[h * dh + (i - h * row)] = r[j];
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ eviction
+struct EvictParams {
+  CacheView c;
+  const float* win;
+  float* wout;
+  long long win_seq, win_head, wout_seq, wout_head;
+  const int* out_table;
+  long long out_stride;
+  int out_pages, wcap;
+  int* new_lens;
+  int* kept;
+  int budget, recent;
+  bool same_weights, in_place;
+};
+
+// Length of sequence s, or -1 (and the error raised) when the table, the weights or the
+// destination cannot hold it.
+__device__ __forceinline__ int evict_length(const EvictParams& p, int s) {
+  const int len = p.c.lens[s];
+  const int n = min(len, p.budget);
+  if (len < 0 || len > min(cache_capacity(p.c.max_pages, p.c.page_size), p.wcap) ||
+      n > cache_capacity(p.out_pages, p.c.page_size)) {
+    if (threadIdx.x == 0) atomicOr(p.c.err, kCacheBadLength);
+    return -1;
+  }
+  return len;
+}
+
+// Order-preserving bits of a weight: larger weight, larger key; -0 as +0, NaN as -infinity.
+__device__ __forceinline__ unsigned weight_key(float w) {
+  if (w != w) w = -__int_as_float(0x7f800000);
+  const unsigned u = __float_as_uint(w + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+constexpr int kSelThreads = 1024;
+constexpr int kSelWarps = kSelThreads / 32;
+
+// Chooses the kept tokens of one (sequence, head) and compacts its weights.  The n - r largest
+// of the first len - r weights are found by radix selection: four passes over 8-bit digits, each
+// narrowing the threshold key.  Then every warp takes a contiguous part of the tokens, counts
+// the kept ones, and writes their slots in order; ties at the threshold go to the first ones.
+__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictParams p) {
+  griddep_launch_dependents();
+  __shared__ unsigned hist[8][256];
+  __shared__ int warp_gt[kSelWarps], warp_eq[kSelWarps];
+  __shared__ unsigned sh_prefix;
+  __shared__ int sh_need;
+  const int s = blockIdx.x / p.c.kv_heads, h = blockIdx.x - s * p.c.kv_heads;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int len = evict_length(p, s);
+  int* kept = p.kept + (long long)blockIdx.x * p.budget;
+  const float* win = p.win + s * p.win_seq + h * p.win_head;
+  float* wout = p.wout + s * p.wout_seq + h * p.wout_head;
+  const int n = len < 0 ? 0 : min(len, p.budget);
+  if (tid == 0 && h == 0) p.new_lens[s] = n;
+  for (int j = n + tid; j < p.budget; j += kSelThreads) kept[j] = -1;
+  if (len <= 0) return;
+  if (n == len) {  // everything stays
+    for (int j = tid; j < n; j += kSelThreads) {
+      kept[j] = j;
+      if (!p.same_weights) wout[j] = win[j];
+    }
+    return;
+  }
+  const int r = min(p.recent, n), old = len - r, need = n - r;
+  // threshold: the need-th largest key of [0, old); `ties` of the keys equal to it are kept
+  unsigned prefix = 0;
+  int ties = need;
+  if (need > 0) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      for (int i = tid; i < 8 * 256; i += kSelThreads) hist[0][i] = 0;
+      __syncthreads();
+      for (int i = tid; i < old; i += kSelThreads) {
+        const unsigned key = weight_key(win[i]);
+        if (shift == 24 || (key >> (shift + 8)) == prefix >> (shift + 8)) atomicAdd(&hist[warp & 7][(key >> shift) & 255], 1u);
+      }
+      __syncthreads();
+      if (warp == 0) {
+        // lane l holds the digits 255 - 8 l .. 248 - 8 l, largest first
+        int cnt[8], sum = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          cnt[j] = 0;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) cnt[j] += hist[c][255 - 8 * lane - j];
+          sum += cnt[j];
+        }
+        int before = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int o = __shfl_up_sync(0xffffffffu, before, d);
+          if (lane >= d) before += o;
+        }
+        before -= sum;  // keys with a larger digit held by lower lanes
+        if (before < ties && before + sum >= ties) {
+          int left = ties - before;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (left > 0 && left <= cnt[j]) {
+              sh_prefix = prefix | (unsigned)(255 - 8 * lane - j) << shift;
+              sh_need = left;
+            }
+            left -= cnt[j];
+          }
+        }
+      }
+      __syncthreads();
+      prefix = sh_prefix;
+      ties = sh_need;
+    }
+  }
+  // contiguous part of each warp, a multiple of 32 tokens
+  const int part = ((len + kSelThreads - 1) / kSelThreads) * 32;
+  const int i0 = warp * part, i1 = min(len, i0 + part);
+  int gt = 0, eq = 0;
+  for (int i = i0 + lane; i - lane < i1; i += 32) {
+    const unsigned key = i < i1 && i < old ? weight_key(win[i]) : 0;
+    const bool more = i < i1 && (i >= old || (need > 0 && key > prefix));
+    const bool same = i < i1 && i < old && need > 0 && key == prefix;
+    gt += __popc(__ballot_sync(0xffffffffu, more));
+    eq += __popc(__ballot_sync(0xffffffffu, same));
+  }
+  if (lane == 0) {
+    warp_gt[warp] = gt;
+    warp_eq[warp] = eq;
+  }
+  __syncthreads();
+  int at = 0, seen = 0;  // kept tokens and threshold keys before this warp's part
+  for (int w = 0; w < warp; ++w) {
+    at += warp_gt[w];
+    seen += warp_eq[w];
+  }
+  at += min(seen, ties);
+  const unsigned below = (1u << lane) - 1;
+  for (int i = i0 + lane; i - lane < i1; i += 32) {
+    const unsigned key = i < i1 && i < old ? weight_key(win[i]) : 0;
+    const bool same = i < i1 && i < old && need > 0 && key == prefix;
+    const unsigned eqs = __ballot_sync(0xffffffffu, same);
+    const bool keep = i < i1 && (i >= old || (need > 0 && key > prefix) || (same && seen + __popc(eqs & below) < ties));
+    const unsigned ks = __ballot_sync(0xffffffffu, keep);
+    if (keep) kept[at + __popc(ks & below)] = i;
+    at += __popc(ks);
+    seen += __popc(eqs);
+  }
+  __syncthreads();
+  // Weights in order.  In place, a block of them is read before any of it is written: slot j
+  // comes from kept[j] >= j, so what a later block reads lies behind what this one writes.
+  for (int j0 = 0; j0 < n; j0 += 4 * kSelThreads) {
+    float w[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int j = j0 + q * kSelThreads + tid;
+      if (j < n) w[q] = win[kept[j]];
+    }
+    if (p.same_weights) __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int j = j0 + q * kSelThreads + tid;
+      if (j < n) wout[j] = w[q];
+    }
+  }
+  __syncthreads();
+  for (int j = n + tid; j < len; j += kSelThreads) wout[j] = 0.0f;
+}
+
+// Offsets of a kept row's source and destination; false (error raised) when a page is bad.
+__device__ __forceinline__ bool evict_offsets(const EvictParams& p, int s, int h, int j, int from, long long* src,
+                                              long long* dst) {
+  const int* row = p.c.table + s * p.c.table_stride;
+  const int* out = p.out_table + s * p.out_stride;
+  const long long a = cache_slot(row, from, p.c.page_size, p.c.num_pages, p.c.page_stride, p.c.token_stride);
+  const long long b = cache_slot(out, j, p.c.page_size, p.c.num_pages, p.c.page_stride, p.c.token_stride);
+  if (a < 0 || b < 0) {
+    atomicOr(p.c.err, kCacheBadPage);
+    return false;
+  }
+  if (!p.in_place && row[j / p.c.page_size] == out[j / p.c.page_size]) {
+    atomicOr(p.c.err, kCacheSamePage);
+    return false;
+  }
+  *src = a + h * p.c.head_stride;
+  *dst = b + h * p.c.head_stride;
+  return true;
+}
+
+constexpr int kMoveRows = 64;  // kept rows of one CTA
+
+// Rows to other pages: every CTA moves 64 kept rows of one (sequence, head), keys and values
+// together, with eight independent loads per thread.
+template <typename U, int ESZ>
+__global__ void __launch_bounds__(256) evict_copy_kernel(const EvictParams p) {
+  griddep_wait();
+  const int s = blockIdx.y / p.c.kv_heads, h = blockIdx.y - s * p.c.kv_heads;
+  const int len = evict_length(p, s);
+  const int n = len < 0 ? 0 : min(len, p.budget);
+  const int j0 = blockIdx.x * kMoveRows;
+  if (j0 >= n) return;
+  __shared__ long long src[kMoveRows], dst[kMoveRows];
+  const int rows = min(kMoveRows, n - j0);
+  if (threadIdx.x < rows) {
+    const int j = j0 + threadIdx.x;
+    if (!evict_offsets(p, s, h, j, p.kept[(long long)blockIdx.y * p.budget + j], &src[threadIdx.x], &dst[threadIdx.x]))
+      src[threadIdx.x] = -1;
+  }
+  __syncthreads();
+  constexpr int PER = sizeof(U) / ESZ;
+  const int row = p.c.dim / PER, total = rows * row;
+  const U* k = static_cast<const U*>(p.c.k);
+  const U* v = static_cast<const U*>(p.c.v);
+  U* ko = static_cast<U*>(p.c.k);
+  U* vo = static_cast<U*>(p.c.v);
+  for (int i0 = threadIdx.x; i0 < total; i0 += 4 * 256) {
+    U a[4], b[4];
+    long long to[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int i = i0 + q * 256;
+      to[q] = -1;
+      if (i < total) {
+        const int j = i / row, e = i - j * row;
+        if (src[j] >= 0) {
+          const long long from = src[j] / PER + e;
+          to[q] = dst[j] / PER + e;
+          a[q] = k[from];
+          b[q] = v[from];
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (to[q] >= 0) {
+        ko[to[q]] = a[q];
+        vo[to[q]] = b[q];
+      }
+  }
+}
+
+// Rows within their own pages: slot j comes from kept[j] >= j, so a CTA that walks the rows in
+// order, reading a block of them before writing any of it, never overwrites what it has still
+// to read.  One CTA takes `slice` units of every row of one pool, so that a (sequence, head) has
+// several.
+template <typename U, int ESZ>
+__global__ void __launch_bounds__(256) evict_shift_kernel(const EvictParams p, int slice) {
+  griddep_wait();
+  const int s = blockIdx.y / p.c.kv_heads, h = blockIdx.y - s * p.c.kv_heads;
+  const int len = evict_length(p, s);
+  if (len <= p.budget) return;
+  const int n = p.budget;
+  constexpr int PER = sizeof(U) / ESZ, Q = 4;
+  const int row = p.c.dim / PER;
+  const int e0 = blockIdx.x * slice, width = min(slice, row - e0);
+  U* pool = static_cast<U*>(blockIdx.z ? p.c.v : p.c.k);
+  const int* kept = p.kept + (long long)blockIdx.y * p.budget;
+  const int per_pass = 256 / slice;  // rows of one pass over the threads
+  const int tr = threadIdx.x / slice, te = threadIdx.x - tr * slice;
+  const bool live = tr < per_pass && te < width;
+  for (int j0 = 0; j0 < n; j0 += Q * per_pass) {
+    U r[Q];
+    long long to[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      const int j = j0 + q * per_pass + tr;
+      to[q] = -1;
+      if (live && j < n) {
+        const int from = kept[j];
+        long long a, b;
+        if (from != j && evict_offsets(p, s, h, j, from, &a, &b)) {
+          r[q] = pool[a / PER + e0 + te];
+          to[q] = b / PER + e0 + te;
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      if (to[q] >= 0) pool[to[q]] = r[q];
+    __syncthreads();
+  }
+}
+
+bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return x < y + nb && y < x + na;
+}
+
+}  // namespace
+
+extern "C" {
+
+__attribute__((visibility("default"))) int spinn_cuda_stream_sync(void* stream) {
+  int dev;
+  int rc = check_stream_device("stream_sync", stream, &dev);
+  if (rc) return rc;
+  unsigned* word = nullptr;
+  rc = decode_error_word(dev, &word);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  unsigned bits = 0;
+  SPINN_CUDA_TRY(cudaMemcpyAsync(&bits, word, sizeof(bits), cudaMemcpyDeviceToHost, st));
+  SPINN_CUDA_TRY(cudaStreamSynchronize(st));
+  if (!bits) return 0;
+  SPINN_CUDA_TRY(cudaMemsetAsync(word, 0, sizeof(bits), st));
+  SPINN_CUDA_TRY(cudaStreamSynchronize(st));
+  if (bits & kLinearTimeout) {
+    set_error("a kernel's bounded wait expired");
+    return SPINN_CUDA_ETIMEOUT;
+  }
+  set_error("paged cache:%s%s%s", bits & kCacheBadPage ? " a page number outside the pool;" : "",
+            bits & kCacheBadLength ? " a length outside its table, weights or rows;" : "",
+            bits & kCacheSamePage ? " an output page that the call reads (in place takes the same table pointer);" : "");
+  return SPINN_CUDA_EINVAL;
+}
+
+__attribute__((visibility("default"))) int spinn_cuda_cache_append(const SpinnCudaCache* cache,
+                                                                   const SpinnCudaPageTable* table,
+                                                                   const SpinnCudaAppend* rows, void* stream) {
+  AppendParams p;
+  int rc = cache_view("cache_append", cache, table, &p.c);
+  if (rc) return rc;
+  SPINN_CHECK_ARG(rows && rows->k && rows->v, "cache_append: k and v are required");
+  SPINN_CHECK_ARG(rows->tokens >= 0, "cache_append: %d tokens", rows->tokens);
+  SPINN_CHECK_ARG(rows->starts || rows->tokens == table->seqs, "cache_append: %d tokens for %d sequences without starts",
+                  rows->tokens, table->seqs);
+  SPINN_CHECK_ARG(rows->k_token_stride >= 0 && rows->k_head_stride >= 0 && rows->v_token_stride >= 0 &&
+                      rows->v_head_stride >= 0,
+                  "cache_append: negative stride");
+  const int es = dtype_bytes(cache->dtype);
+  SPINN_CHECK_ARG(((uintptr_t)rows->k | (uintptr_t)rows->v) % es == 0 && (uintptr_t)rows->starts % 4 == 0,
+                  "cache_append: misaligned pointer");
+  int dev;
+  rc = check_stream_device("cache_append", stream, &dev);
+  if (rc) return rc;
+  if (rows->tokens == 0) return 0;
+  rc = decode_error_word(dev, &p.c.err);
+  if (rc) return rc;
+  p.k = rows->k;
+  p.v = rows->v;
+  p.k_tok = rows->k_token_stride;
+  p.k_head = rows->k_head_stride;
+  p.v_tok = rows->v_token_stride;
+  p.v_head = rows->v_head_stride;
+  p.starts = rows->starts;
+  p.tokens = rows->tokens;
+  const int per = 16 / es;
+  const bool vec = cache_vec16(p.c, es) && aligned16(p.k) && aligned16(p.v) && p.k_tok % per == 0 &&
+                   p.k_head % per == 0 && p.v_tok % per == 0 && p.v_head % per == 0;
+  const unsigned blocks = (unsigned)((2ll * p.tokens + 7) / 8);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (vec && es == 2)
+    append_kernel<uint4, 2><<<blocks, 256, 0, st>>>(p);
+  else if (vec)
+    append_kernel<uint4, 4><<<blocks, 256, 0, st>>>(p);
+  else if (es == 2)
+    append_kernel<uint16_t, 2><<<blocks, 256, 0, st>>>(p);
+  else
+    append_kernel<uint32_t, 4><<<blocks, 256, 0, st>>>(p);
+  SPINN_CUDA_TRY(cudaGetLastError());
+  return 0;
+}
+
+__attribute__((visibility("default"))) int spinn_cuda_cache_evict(const SpinnCudaCache* cache,
+                                                                  const SpinnCudaPageTable* table,
+                                                                  const SpinnCudaEvict* e, void* stream) {
+  EvictParams p;
+  int rc = cache_view("cache_evict", cache, table, &p.c);
+  if (rc) return rc;
+  SPINN_CHECK_ARG(e && e->weights_in && e->weights_out && e->out_pages && e->new_lens && e->kept,
+                  "cache_evict: weights, out_pages, new_lens and kept are required");
+  SPINN_CHECK_ARG(e->budget > 0 && e->recent >= 0, "cache_evict: budget %d, recent %d", e->budget, e->recent);
+  SPINN_CHECK_ARG(e->out_max_pages > 0 && e->out_row_stride >= 0 && e->weights_capacity > 0,
+                  "cache_evict: bad output table or weights");
+  SPINN_CHECK_ARG(e->win_seq_stride >= 0 && e->win_head_stride >= 0 && e->wout_seq_stride >= 0 &&
+                      e->wout_head_stride >= 0,
+                  "cache_evict: negative stride");
+  SPINN_CHECK_ARG(e->new_lens != table->lens, "cache_evict: new_lens must not be the lengths it is read from");
+  SPINN_CHECK_ARG((((uintptr_t)e->weights_in | (uintptr_t)e->weights_out | (uintptr_t)e->out_pages |
+                    (uintptr_t)e->new_lens | (uintptr_t)e->kept) & 3) == 0,
+                  "cache_evict: misaligned pointer");
+  const long long pairs = (long long)table->seqs * cache->kv_heads;
+  SPINN_CHECK_ARG(pairs <= 65535, "cache_evict: %lld (sequence, head) pairs, at most 65535", pairs);
+  p.in_place = e->out_pages == table->pages;
+  SPINN_CHECK_ARG(!p.in_place || e->out_row_stride == table->row_stride,
+                  "cache_evict: in place, the output table's stride must be the table's");
+  p.same_weights = e->weights_in == e->weights_out;
+  const size_t wi = 4 * ((table->seqs - 1) * (size_t)e->win_seq_stride + (cache->kv_heads - 1) * (size_t)e->win_head_stride +
+                         e->weights_capacity);
+  const size_t wo = 4 * ((table->seqs - 1) * (size_t)e->wout_seq_stride +
+                         (cache->kv_heads - 1) * (size_t)e->wout_head_stride + e->weights_capacity);
+  SPINN_CHECK_ARG(p.same_weights ? e->win_seq_stride == e->wout_seq_stride && e->win_head_stride == e->wout_head_stride
+                                 : !overlap(e->weights_in, wi, e->weights_out, wo),
+                  "cache_evict: weights_out must be weights_in itself or apart from it");
+  int dev;
+  rc = check_stream_device("cache_evict", stream, &dev);
+  if (rc) return rc;
+  rc = decode_error_word(dev, &p.c.err);
+  if (rc) return rc;
+  p.win = e->weights_in;
+  p.wout = e->weights_out;
+  p.win_seq = e->win_seq_stride;
+  p.win_head = e->win_head_stride;
+  p.wout_seq = e->wout_seq_stride;
+  p.wout_head = e->wout_head_stride;
+  p.out_table = e->out_pages;
+  p.out_stride = e->out_row_stride;
+  p.out_pages = e->out_max_pages;
+  p.wcap = e->weights_capacity;
+  p.new_lens = e->new_lens;
+  p.kept = e->kept;
+  p.budget = e->budget;
+  p.recent = e->recent;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  evict_select_kernel<<<(unsigned)pairs, kSelThreads, 0, st>>>(p);
+  SPINN_CUDA_TRY(cudaGetLastError());
+  const int es = dtype_bytes(cache->dtype);
+  const bool vec = cache_vec16(p.c, es);
+  const int units = vec ? p.c.dim * es / 16 : p.c.dim;  // copied units of a row
+  if (p.in_place) {
+    // 64 bytes of a row per CTA keep DRAM bursts whole
+    const int slice = std::min(units, vec ? 4 : 64 / es);
+    const dim3 grid((units + slice - 1) / slice, (unsigned)pairs, 2);
+    if (vec && es == 2) return launch_dependent(evict_shift_kernel<uint4, 2>, grid, 256, 0, st, p, slice);
+    if (vec) return launch_dependent(evict_shift_kernel<uint4, 4>, grid, 256, 0, st, p, slice);
+    if (es == 2) return launch_dependent(evict_shift_kernel<uint16_t, 2>, grid, 256, 0, st, p, slice);
+    return launch_dependent(evict_shift_kernel<uint32_t, 4>, grid, 256, 0, st, p, slice);
+  }
+  const int most = std::min(std::min(p.budget, p.wcap), cache_capacity(p.c.max_pages, p.c.page_size));
+  const dim3 grid((most + kMoveRows - 1) / kMoveRows, (unsigned)pairs, 1);
+  if (vec && es == 2) return launch_dependent(evict_copy_kernel<uint4, 2>, grid, 256, 0, st, p);
+  if (vec) return launch_dependent(evict_copy_kernel<uint4, 4>, grid, 256, 0, st, p);
+  if (es == 2) return launch_dependent(evict_copy_kernel<uint16_t, 2>, grid, 256, 0, st, p);
+  return launch_dependent(evict_copy_kernel<uint32_t, 4>, grid, 256, 0, st, p);
+}
+
+__attribute__((visibility("default"))) int64_t spinn_cuda_diag_cache_slot(const int32_t* row, int max_pages, int pos,
+                                                                          int page_size, int num_pages,
+                                                                          int64_t page_stride, int64_t token_stride) {
+  if (!row || max_pages <= 0 || page_size <= 0 || pos < 0 || pos >= cache_capacity(max_pages, page_size)) return -2;
+  return cache_slot(row, pos, page_size, num_pages, page_stride, token_stride);
+}
+
+__attribute__((visibility("default"))) int spinn_cuda_diag_attention_share(int64_t units, int workers, int worker,
+                                                                           int64_t unit, int64_t* out3) {
+  SPINN_CHECK_ARG(out3 && units > 0 && workers > 0 && worker >= 0 && worker < workers && unit >= 0 && unit < units,
+                  "spinn_cuda_diag_attention_share: invalid arguments");
+  out3[0] = attn_start(units, workers, worker);
+  out3[1] = attn_start(units, workers, worker + 1);
+  out3[2] = attn_owner(units, workers, unit);
+  return 0;
+}
+
+}  // extern "C"
+}  // namespace spinn

@@ -1,0 +1,69 @@
+// cache.h -- the paged key-value cache shared by cache.cu (append, eviction) and attention.cu:
+// where a token's row lies, and how one attention launch splits its work.  The arithmetic is
+// host code as well, so that the CPU tests run what the kernels run.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/spinn_cuda.h"
+
+namespace spinn {
+
+// Deferred errors of the decoder-serving operators, raised by a kernel that skips the access instead of
+// making it (spinn_cuda_stream_sync reports and clears them).
+enum CacheErr : unsigned { kCacheBadPage = 1, kCacheBadLength = 2, kCacheSamePage = 4, kLinearTimeout = 8 };
+
+// The pools and their page table as the kernels see them.  Strides are in elements.
+struct CacheView {
+  void* k;
+  void* v;
+  long long page_stride, token_stride, head_stride;
+  int num_pages, page_size, kv_heads, dim;
+  const int* table;
+  long long table_stride;
+  int max_pages, seqs;
+  const int* lens;
+  unsigned* err;  // deferred error word of the device
+};
+
+// Tokens that a table row can hold (lengths are 32-bit).
+__host__ __device__ inline int cache_capacity(int max_pages, int page_size) {
+  const long long c = (long long)max_pages * page_size;
+  return c > 0x7fffffffLL ? 0x7fffffff : (int)c;
+}
+
+// Element offset of token `pos` in either pool (head 0) through the table row `row`, or -1 when
+// its page lies outside the pool.  pos must be within the row's capacity.  64-bit: a pool of
+// more than 2^31 elements is ordinary.
+__host__ __device__ inline long long cache_slot(const int* row, int pos, int page_size, int num_pages,
+                                                long long page_stride, long long token_stride) {
+  const int blk = (int)((unsigned)pos / (unsigned)page_size);
+  const int page = row[blk];
+  if (page < 0 || page >= num_pages) return -1;
+  return (long long)page * page_stride + (long long)(pos - blk * page_size) * token_stride;
+}
+
+// Attention's work: `units` tiles of tokens in the order (sequence, head block, tile), dealt to
+// `workers` CTAs in equal contiguous shares.  Worker w has [attn_start(w), attn_start(w + 1)).
+__host__ __device__ inline long long attn_start(long long units, int workers, int w) {
+  return units * w / workers;
+}
+// The worker whose share holds unit u: the last w with floor(units * w / workers) <= u, i.e. the
+// last w below (u + 1) * workers / units.
+__host__ __device__ inline int attn_owner(long long units, int workers, long long u) {
+  return (int)(((u + 1) * workers + units - 1) / units) - 1;
+}
+
+// Host-side checks common to the cache entry points; fills `v`.
+int cache_view(const char* who, const SpinnCudaCache* c, const SpinnCudaPageTable* t, CacheView* v);
+// The current device when `stream` belongs to it, an error otherwise.
+int check_stream_device(const char* who, void* stream, int* device);
+// 16-byte vector access possible: `bytes`-sized elements, pointers and strides (elements).
+bool cache_vec16(const CacheView& v, int bytes);
+int dtype_bytes(int dtype);
+
+// The current device's deferred error word (device memory; CacheErr bits, kLinearTimeout).
+int decode_error_word(int device, unsigned** word);
+
+}  // namespace spinn

@@ -16,6 +16,9 @@ LIB_PATH = os.path.join(HERE, "libspinn_cuda.so")
 OK, EINVAL, ENOMEM, ECUDA, EUNSUPPORTED, ETIMEOUT, EFORMAT, ESTATE = 0, -1, -2, -3, -4, -5, -6, -7
 PLAN_NO_GRAPH, PLAN_PROFILE, PLAN_NO_ROUND, PLAN_WINOGRAD, PLAN_KEEP, PLAN_NO_FUSE = 1, 2, 4, 8, 16, 32
 
+# Element types of the decoder-serving operators (ENNF / ONNX codes)
+FP32, FP16, BF16 = 1, 10, 16
+
 # ENNF operator codes (SPINN/ennf_op_types.h:79,134,135)
 OP_CONV, OP_GEMM, OP_MATMUL = 60, 160, 161
 
@@ -62,6 +65,17 @@ _SIGS = {
     "spinn_cuda_matmul": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_uint16,
                                          ctypes.c_void_p, ctypes.c_int]),
     "spinn_cuda_conv2d_noalloc": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_int] * 12 + [ctypes.c_void_p]),
+    # descriptors are passed as packed bytes
+    "spinn_cuda_stream_sync": (ctypes.c_int, [ctypes.c_void_p]),
+    "spinn_cuda_cache_append": (ctypes.c_int, [ctypes.c_char_p] * 3 + [ctypes.c_void_p]),
+    "spinn_cuda_paged_attention_workspace": (ctypes.c_size_t, [ctypes.c_char_p] * 3),
+    "spinn_cuda_paged_attention": (ctypes.c_int, [ctypes.c_char_p] * 3 + [ctypes.c_void_p, ctypes.c_size_t,
+                                                                          ctypes.c_void_p]),
+    "spinn_cuda_cache_evict": (ctypes.c_int, [ctypes.c_char_p] * 3 + [ctypes.c_void_p]),
+    "spinn_cuda_diag_cache_slot": (ctypes.c_int64, [ctypes.POINTER(ctypes.c_int32)] + [ctypes.c_int] * 4 +
+                                   [ctypes.c_int64] * 2),
+    "spinn_cuda_diag_attention_share": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int64,
+                                                       ctypes.POINTER(ctypes.c_int64)]),
     "spinn_cuda_load": (ctypes.c_void_p, [ctypes.c_char_p]),
     "spinn_cuda_load_buffer": (ctypes.c_void_p, [ctypes.c_void_p, ctypes.c_size_t]),
     "spinn_cuda_plan": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_int]),

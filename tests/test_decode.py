@@ -1,0 +1,187 @@
+"""Decoder-serving operators without a GPU: argument checks of the C entry points (which come
+before any CUDA call), of the Python calls, and the host arithmetic that the kernels share."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from spinn_b200 import lib, runtime
+
+BUF = ctypes.create_string_buffer(1 << 16)  # never dereferenced: every call here is refused
+P = (ctypes.addressof(BUF) + 255) & ~255
+
+
+def cache(**kw):
+    f = dict(k=P, v=P, ps=16 * 2 * 64, ts=2 * 64, hs=64, dtype=lib.BF16, pages=9, page=16, heads=2, dim=64)
+    f.update(kw)
+    return runtime._CACHE.pack(f["k"], f["v"], f["ps"], f["ts"], f["hs"], f["dtype"], f["pages"], f["page"],
+                               f["heads"], f["dim"], 0)
+
+
+def table(**kw):
+    f = dict(pages=P, lens=P, stride=4, seqs=3, wide=4)
+    f.update(kw)
+    return runtime._TABLE.pack(f["pages"], f["lens"], f["stride"], f["seqs"], f["wide"])
+
+
+def refused(fn, *args, match):
+    rc = getattr(lib.lib(), fn)(*args)
+    assert rc == lib.EINVAL and match in lib.last_error(), (rc, lib.last_error())
+
+
+BAD_CACHES = [(dict(k=0), "null"), (dict(v=0), "null"), (dict(dtype=7), "type 7"), (dict(dtype=0), "type 0"),
+              (dict(pages=0), "geometry"), (dict(page=0), "geometry"), (dict(page=-16), "geometry"),
+              (dict(heads=0), "geometry"), (dict(heads=65536), "geometry"), (dict(dim=0), "head_dim"),
+              (dict(dim=257), "head_dim"), (dict(ts=-1), "stride"), (dict(k=P + 1), "misaligned")]
+BAD_TABLES = [(dict(pages=0), "null"), (dict(lens=0), "null"), (dict(seqs=0), "page table"), (dict(wide=0), "page table"),
+              (dict(stride=-4), "page table"), (dict(lens=P + 2), "misaligned")]
+
+
+def append(**kw):
+    f = dict(k=P, v=P, starts=0, tokens=3, ks=128)
+    f.update(kw)
+    return runtime._APPEND.pack(f["k"], f["v"], f["ks"], 64, 128, 64, f["starts"], f["tokens"], 0)
+
+
+def attention(**kw):
+    f = dict(q=P, y=P, win=0, wout=0, cap=0, q_heads=4, qs=256, wis=0, wos=0)
+    f.update(kw)
+    return runtime._ATTENTION.pack(f["q"], f["y"], f["qs"], 64, 256, 64, f["win"], f["wout"], f["wis"], 0, f["wos"], 0,
+                                   f["cap"], f["q_heads"], 0.125, 0)
+
+
+def evict(**kw):
+    f = dict(win=P, wout=P + 8192, out=P + 256, stride=4, wide=4, cap=64, new=P + 64, kept=P + 128, budget=16, recent=0,
+             wis=128, wos=128)
+    f.update(kw)
+    return runtime._EVICT.pack(f["win"], f["wout"], f["wis"], 64, f["wos"], 64, f["out"], f["stride"], f["wide"],
+                               f["cap"], f["new"], f["kept"], f["budget"], f["recent"])
+
+
+@pytest.mark.parametrize("kw,match", BAD_CACHES)
+def test_bad_caches_are_refused(kw, match):
+    refused("spinn_cuda_cache_append", cache(**kw), table(), append(), None, match=match)
+    refused("spinn_cuda_paged_attention", cache(**kw), table(), attention(), P, 1 << 15, None, match=match)
+    refused("spinn_cuda_cache_evict", cache(**kw), table(), evict(), None, match=match)
+
+
+@pytest.mark.parametrize("kw,match", BAD_TABLES)
+def test_bad_tables_are_refused(kw, match):
+    refused("spinn_cuda_cache_append", cache(), table(**kw), append(), None, match=match)
+    refused("spinn_cuda_paged_attention", cache(), table(**kw), attention(), P, 1 << 15, None, match=match)
+    refused("spinn_cuda_cache_evict", cache(), table(**kw), evict(), None, match=match)
+
+
+@pytest.mark.parametrize("kw,match", [(dict(k=0), "required"), (dict(tokens=-1), "tokens"), (dict(tokens=5), "without starts"),
+                                      (dict(ks=-1), "stride"), (dict(k=P + 1), "misaligned"),
+                                      (dict(starts=P + 1), "misaligned")])
+def test_append_refusals(kw, match):
+    refused("spinn_cuda_cache_append", cache(), table(), append(**kw), None, match=match)
+
+
+@pytest.mark.parametrize("kw,match", [(dict(q=0), "required"), (dict(y=0), "required"), (dict(q_heads=3), "multiple"),
+                                      (dict(q_heads=0), "multiple"), (dict(qs=-1), "stride"), (dict(y=P + 1), "misaligned"),
+                                      (dict(win=P), "without weights_out"), (dict(wout=P), "geometry"),
+                                      (dict(wout=P, cap=64, q_heads=34), "at most 16"),
+                                      (dict(wout=P, win=P, cap=64, wis=64, wos=128), "in place")])
+def test_attention_refusals(kw, match):
+    refused("spinn_cuda_paged_attention", cache(), table(), attention(**kw), P, 1 << 15, None, match=match)
+
+
+def test_attention_weights_take_fewer_heads_in_fp32():
+    refused("spinn_cuda_paged_attention", cache(dtype=lib.FP32), table(), attention(wout=P, cap=64, q_heads=18), P, 1 << 15,
+            None, match="at most 8")
+
+
+@pytest.mark.parametrize("kw,match", [(dict(win=0), "required"), (dict(kept=0), "required"), (dict(budget=0), "budget"),
+                                      (dict(recent=-1), "budget"), (dict(wide=0), "output table"),
+                                      (dict(cap=0), "output table"), (dict(new=P), "lengths"), (dict(wis=-1), "stride"),
+                                      (dict(out=P, stride=8), "in place"), (dict(wout=P + 16), "apart"),
+                                      (dict(wout=P, wos=64), "apart"), (dict(kept=P + 2), "misaligned")])
+def test_evict_refusals(kw, match):
+    refused("spinn_cuda_cache_evict", cache(), table(), evict(**kw), None, match=match)
+
+
+def test_evict_refuses_more_pairs_than_a_grid_has():
+    refused("spinn_cuda_cache_evict", cache(heads=4096), table(seqs=17), evict(wis=0, wos=0, wout=P + (1 << 20) * 4), None,
+            match="65535")
+
+
+# ------------------------------------------------------------------ Python calls
+def test_python_calls_refuse_host_tensors():
+    torch = pytest.importorskip("torch")
+    k = torch.zeros(4, 16, 2, 64)
+    t, n = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    q = torch.zeros(1, 2, 64)
+    w = torch.zeros(1, 2, 32)
+    with pytest.raises(TypeError, match="CUDA"):
+        runtime.cache_append(q, q, k, k, t, n)
+    with pytest.raises(TypeError, match="CUDA"):
+        runtime.paged_attention(q, k, k, t, n, q)
+    with pytest.raises(TypeError, match="CUDA"):
+        runtime.cache_evict(k, k, t, n, w, w, t, n, n, 4)
+
+
+def test_python_descriptors_check_shapes_and_types():
+    torch = pytest.importorskip("torch")
+    runtime._torch_module()
+    k = torch.zeros(4, 16, 2, 64)
+    with pytest.raises(ValueError, match="one shape"):
+        runtime._cache_desc("x", k, k[..., :32])
+    with pytest.raises(ValueError, match="one shape"):
+        runtime._cache_desc("x", k, torch.zeros(4, 2, 16, 64).transpose(1, 2))
+    with pytest.raises(TypeError, match="float64"):
+        runtime._cache_desc("x", k.double(), k.double())
+    with pytest.raises(ValueError, match="contiguous"):
+        runtime._cache_desc("x", k[..., ::2], k[..., ::2])
+    t = torch.zeros(3, 5, dtype=torch.int32)
+    with pytest.raises(TypeError, match="int32"):
+        runtime._table_desc("x", t.long(), t[:, 0])
+    with pytest.raises(ValueError, match="lens"):
+        runtime._table_desc("x", t, torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(ValueError, match="contiguous"):
+        runtime._table_desc("x", t.t(), torch.zeros(5, dtype=torch.int32))
+    with pytest.raises(TypeError, match="float32"):
+        runtime._weights("x", "weights", torch.zeros(1, 2, 3, dtype=torch.float16), 1, 2)
+    with pytest.raises(TypeError, match="type"):
+        runtime._rows("x", "q", torch.zeros(1, 2, 64, dtype=torch.float16), k, (1, 2, 64))
+
+
+# ------------------------------------------------------------------ shared host arithmetic
+def slot(row, pos, page=16, pages=9, ps=2048, ts=128):
+    r = np.asarray(row, np.int32)
+    return lib.lib().spinn_cuda_diag_cache_slot(r.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)), len(r), pos, page, pages,
+                                                ps, ts)
+
+
+def test_slots():
+    row = [3, 8, 0]
+    for pos in range(48):
+        assert slot(row, pos) == row[pos // 16] * 2048 + pos % 16 * 128
+    assert slot(row, 48) == -2 and slot(row, -1) == -2
+    for bad in (-1, 9, 2 ** 31 - 1, -2 ** 31):
+        assert slot([3, bad, 0], 16) == -1 and slot([3, bad, 0], 15) == 3 * 2048 + 15 * 128
+    # offsets past 32 bits, odd page sizes
+    assert slot([2 ** 20], 5, page=7, pages=2 ** 20 + 1, ps=7 * 8 * 128, ts=1024) == 2 ** 20 * 7168 + 5 * 1024
+    assert slot([0, 1], 3, page=3, pages=2, ps=30, ts=10) == 30
+
+
+def test_attention_shares_cover_the_work_once():
+    L = lib.lib()
+    out = (ctypes.c_int64 * 3)()
+    rng = np.random.default_rng(0)
+    for units, workers in [(1, 296), (5, 3), (296, 296), (295, 296), (297, 296), (7, 1), (2 ** 33 + 5, 296)] + \
+            [(int(rng.integers(1, 5000)), int(rng.integers(1, 300))) for _ in range(40)]:
+        starts = []
+        for w in range(workers):
+            assert L.spinn_cuda_diag_attention_share(units, workers, w, 0, out) == 0
+            starts.append((out[0], out[1]))
+        assert starts[0][0] == 0 and starts[-1][1] == units
+        assert all(a[1] == b[0] for a, b in zip(starts, starts[1:]))
+        sizes = [b - a for a, b in starts]
+        assert max(sizes) - min(sizes) <= 1
+        for u in {0, units - 1, units // 2, *(int(x) for x in rng.integers(0, units, 20))}:
+            L.spinn_cuda_diag_attention_share(units, workers, 0, u, out)
+            a, b = starts[out[2]]
+            assert a <= u < b
+    assert L.spinn_cuda_diag_attention_share(0, 1, 0, 0, out) == lib.EINVAL
