@@ -142,7 +142,8 @@ int spinn_cuda_conv2d_noalloc(const float *x, const float *w, const float *bias,
 
 /* Operators of a decoding step on device memory, queued on the caller's stream: a paged key-value
  * cache with its append, its attention of one new token per sequence and its eviction by
- * accumulated attention weight.  The reference has no counterpart.
+ * accumulated attention weight, and a 16-bit linear layer with its epilogue fused.  The reference
+ * has no counterpart.
  *
  * Every pointer is device memory of the current device.  `stream` (NULL = the legacy default
  * stream) must belong to the current device; nothing is waited for and nothing is allocated, so
@@ -246,6 +247,26 @@ typedef struct {
 } SpinnCudaEvict;
 int spinn_cuda_cache_evict(const SpinnCudaCache *cache, const SpinnCudaPageTable *table, const SpinnCudaEvict *e,
                            void *stream);
+
+/* Linear layer: y = act(x w^T + bias) + residual, x [m][k], w [n][k], y and residual [m][n], bias
+ * [n], all of one 16-bit type (dtype SPINN_CUDA_FP16 or _BF16; the fp32 form is
+ * spinn_cuda_gemm).  Rows are contiguous, row strides in elements.  Products accumulate in fp32
+ * and y is rounded once.  bias and residual may be NULL; y may be the residual itself.
+ * act: the ENNF fused-act codes 0 (none), 1 (ReLU), 3 (SiLU), and 6 (GELU, by erf), 7 (GELU, by
+ * tanh); unlike the convolutions' 4 and 5 the residual is added after the activation. */
+#define SPINN_CUDA_ACT_GELU 6
+#define SPINN_CUDA_ACT_GELU_TANH 7
+typedef struct {
+    const void *x, *w, *bias, *residual;
+    void *y;
+    int64_t x_stride, w_stride, residual_stride, y_stride;
+    int32_t m, n, k;
+    int32_t dtype;
+    int32_t act;
+    int32_t reserved; /* 0 */
+} SpinnCudaLinear;
+size_t spinn_cuda_linear_workspace(const SpinnCudaLinear *l);
+int spinn_cuda_linear(const SpinnCudaLinear *l, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Diagnostics (host only): element offset of token `pos` of a table row of max_pages entries in a
  * contiguous pool, or a negative value when its page is outside the pool or pos outside the

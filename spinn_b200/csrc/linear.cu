@@ -1,0 +1,713 @@
+// linear.cu -- y = act(x w^T + bias) + residual in 16-bit types, accumulated in fp32.
+//
+// Two kernels, by the number of rows m of x:
+//
+// * linear_rows_kernel, m <= 16 (single tokens, small decoding batches): bound by reading w once.
+//   No staging: the fragments of mma.sync come straight from global memory, 16 bytes per lane,
+//   with k permuted the same way in both operands so that a lane's 16 contiguous bytes are its
+//   fragment.  Any alignment.
+//
+// * linear_tile_kernel: tcgen05 with TMA-fed swizzled stages.  The rows of w are the MMA's rows
+//   (TMEM lanes) and the rows of x its columns, i.e. it computes y^T tiles: a warp that drains
+//   its 32 lanes then holds 32 consecutive outputs of one row of y, so residual and y are read
+//   and written in whole segments at any alignment, without a transposing stage.  Few rows of x
+//   only make the MMA narrower, so the same kernel serves decoding batches, where k is split
+//   over a cluster whose CTAs add their partial tiles through distributed shared memory.
+//   Operands whose rows are not 16-byte aligned are first copied to an aligned pitch.
+#include <algorithm>
+#include <type_traits>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "cache.h"
+#include "internal.h"
+#include "launch.h"
+#include "ptx.cuh"
+
+namespace spinn {
+namespace {
+
+constexpr uint64_t kTimeoutNs = 4000000000ull;  // bounded barrier waits
+constexpr uint64_t kDrainNs = 1000000000ull;
+constexpr int kRowsMax = 16;  // rows of x that linear_rows_kernel takes
+
+struct LinearParams {
+  const void* x;
+  const void* w;
+  const void* bias;
+  const void* res;
+  void* y;
+  long long ldx, ldw, ldr, ldy;
+  int m, n, k;
+  int act;
+  int num_kb, tiles_m, tiles_n, num_tiles;
+  bool vec;
+  unsigned* err;
+};
+
+template <typename T>
+__device__ __forceinline__ float to_float(T x) {
+  if constexpr (std::is_same<T, __half>::value)
+    return __half2float(x);
+  else
+    return __bfloat162float(x);
+}
+template <typename T>
+__device__ __forceinline__ T round_to(float x) {
+  if constexpr (std::is_same<T, __half>::value)
+    return __float2half_rn(x);
+  else
+    return __float2bfloat16_rn(x);
+}
+
+// The activations of the fp32 accumulator.  SiLU and the tanh form share v / (1 + e^-z): the tanh
+// form is 0.5 v (1 + tanh u) = v / (1 + e^(-2 u)).  __expf's error (2 ulp plus 2^-22 |z|) is far
+// below the rounding of y.
+__device__ __forceinline__ float activate(float v, int act) {
+  switch (act) {
+    case 1:
+      return v < 0.0f ? 0.0f : v;
+    case 3:
+      return v / (1.0f + __expf(-v));
+    case SPINN_CUDA_ACT_GELU:
+      return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+    case SPINN_CUDA_ACT_GELU_TANH: {
+      const float u = 1.5957691216057308f * (v + 0.044715f * v * v * v);  // 2 sqrt(2 / pi) (...)
+      return v / (1.0f + __expf(-u));
+    }
+    default:
+      return v;
+  }
+}
+
+// ------------------------------------------------------------------ few rows
+template <typename T>
+__device__ __forceinline__ void mma_rows(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Elements k .. k + 7 of a row (zeros past `end`; nothing is read where !row).
+template <bool VEC>
+__device__ __forceinline__ uint4 load8(const uint16_t* row, bool live, int k, int end) {
+  uint4 r = make_uint4(0, 0, 0, 0);
+  if (!live || k >= end) return r;
+  if (VEC && k + 8 <= end) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  uint32_t h[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) h[i] = k + i < end ? __ldg(row + k + i) : 0;
+  r.x = h[0] | h[1] << 16;
+  r.y = h[2] | h[3] << 16;
+  r.z = h[4] | h[5] << 16;
+  r.w = h[6] | h[7] << 16;
+  return r;
+}
+
+constexpr int kRowWarps = 8;
+
+// CTA: 16 rows of w, all rows of x (NT blocks of 8); its warps take interleaved 128-element
+// chunks of k and are summed in order through shared memory.
+template <typename T, int NT, bool VEC>
+__global__ void __launch_bounds__(kRowWarps * 32) linear_rows_kernel(const LinearParams p) {
+  __shared__ float part[kRowWarps][NT * 8][16];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n0 = blockIdx.x * 16, r = lane >> 2, q = lane & 3;
+  const uint16_t* w0 = static_cast<const uint16_t*>(p.w) + (long long)(n0 + r) * p.ldw;
+  const uint16_t* w1 = w0 + 8 * p.ldw;
+  const bool live0 = n0 + r < p.n, live1 = n0 + r + 8 < p.n;
+  float acc[NT][4];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.0f;
+  constexpr int U = 4;  // 32-element steps in flight
+  for (int k0 = warp * 32 * U; k0 < p.k; k0 += kRowWarps * 32 * U) {
+    uint4 a[U], b[U], x[U][NT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * 32 + q * 8;
+      a[u] = load8<VEC>(w0, live0, k, p.k);
+      b[u] = load8<VEC>(w1, live1, k, p.k);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        x[u][t] = load8<VEC>(static_cast<const uint16_t*>(p.x) + (t * 8 + r) * p.ldx, t * 8 + r < p.m, k, p.k);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        mma_rows<T>(acc[t], a[u].x, b[u].x, a[u].y, b[u].y, x[u][t].x, x[u][t].y);
+        mma_rows<T>(acc[t], a[u].z, b[u].z, a[u].w, b[u].w, x[u][t].z, x[u][t].w);
+      }
+  }
+  // accumulator: rows r and r + 8 of w, tokens 2 q and 2 q + 1
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    part[warp][t * 8 + 2 * q][r] = acc[t][0];
+    part[warp][t * 8 + 2 * q + 1][r] = acc[t][1];
+    part[warp][t * 8 + 2 * q][r + 8] = acc[t][2];
+    part[warp][t * 8 + 2 * q + 1][r + 8] = acc[t][3];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < NT * 8 * 16; i += kRowWarps * 32) {
+    const int row = i >> 4, n = n0 + (i & 15);
+    if (row >= p.m || n >= p.n) continue;
+    float v = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kRowWarps; ++s) v += part[s][row][i & 15];
+    if (p.bias) v += to_float(static_cast<const T*>(p.bias)[n]);
+    v = activate(v, p.act);
+    if (p.res) v += to_float(static_cast<const T*>(p.res)[row * p.ldr + n]);
+    static_cast<T*>(p.y)[row * p.ldy + n] = round_to<T>(v);
+  }
+}
+
+// ------------------------------------------------------------------ rows to an aligned pitch
+// dst[r][0 .. pitch) = src[r][0 .. k), zeros behind.  One launch for both operands.
+struct PitchParams {
+  const uint16_t* src[2];
+  uint16_t* dst[2];
+  long long ld[2];
+  int rows[2];
+  int k, pitch;
+};
+__global__ void __launch_bounds__(256) pitch_kernel(const PitchParams p) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const int o = blockIdx.y;
+  for (int r = blockIdx.x; r < p.rows[o]; r += gridDim.x) {
+    const uint16_t* s = p.src[o] + r * p.ld[o];
+    uint16_t* d = p.dst[o] + (long long)r * p.pitch;
+    for (int c = threadIdx.x * 8; c < p.pitch; c += 256 * 8) {
+      uint32_t h[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) h[i] = c + i < p.k ? s[c + i] : 0;
+      *reinterpret_cast<uint4*>(d + c) =
+          make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ tiles on tcgen05
+// kind::f16: D fp32 [4,6) = 1, A and B type 0 fp16 / 1 bf16 at [7,10) and [10,13), both K-major.
+template <typename T>
+__host__ __device__ constexpr uint32_t make_idesc_16(uint32_t M, uint32_t N) {
+  constexpr uint32_t f = std::is_same<T, __half>::value ? 0 : 1;
+  return (1u << 4) | (f << 7) | (f << 10) | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+__device__ __forceinline__ void umma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ bool warp_wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, kTimeoutNs));
+}
+__device__ __forceinline__ bool warp_abort(volatile int* abort) { return __any_sync(0xffffffffu, *abort != 0); }
+
+constexpr int kTileThreads = 384;  // producer, MMA, TMEM and a spare warp, eight epilogue warps
+
+// BN: rows of x of a tile.  PAIR 2: a CTA pair works on 256 rows of w with one cta_group::2 MMA
+// stream, each CTA holding its 128 rows of w and half of the rows of x.  SPL: the CTAs of a
+// cluster share one tile and split its k.
+template <int BN_, int PAIR_, bool SPL_>
+struct LinCfg {
+  static constexpr int BN = BN_, PAIR = PAIR_;
+  static constexpr bool SPL = SPL_;
+  static constexpr int BK = 64;                     // 128-byte rows: one swizzle span
+  static constexpr int A_STAGE = 128 * 128, B_STAGE = BN / PAIR * 128, STAGE = A_STAGE + B_STAGE;
+  static constexpr int FIT = (222 * 1024) / STAGE;
+  static constexpr int STAGES = FIT > 10 ? 10 : FIT;
+  static constexpr int NACC = SPL ? 1 : 2;          // accumulators: the epilogue drains one while the other fills
+  static constexpr int COLS = NACC * BN < 32 ? 32 : NACC * BN;
+  static constexpr int SMEM = STAGES * STAGE + 512 + 1024;
+  static_assert(COLS <= 512, "TMEM");
+  static_assert(!SPL || (PAIR == 1 && STAGES * STAGE >= BN * 128 * 4), "partial tiles reuse the stages");
+};
+
+template <typename T, typename C>
+__global__ void __launch_bounds__(kTileThreads, 1)
+    linear_tile_kernel(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX,
+                       const LinearParams p) {
+  constexpr int BN = C::BN, PAIR = C::PAIR, STAGES = C::STAGES, NACC = C::NACC;
+  constexpr bool SPL = C::SPL;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + STAGES * C::A_STAGE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * C::STAGE);
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;
+  uint64_t* tempty = tfull + NACC;
+  uint64_t* drain = tempty + NACC;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR == 2 || SPL ? cluster_ctarank() : 0;
+  const uint32_t splits = SPL ? cluster_size() : 1;
+  const int unit0 = SPL ? blockIdx.x / splits : blockIdx.x / PAIR;
+  const int step = SPL ? p.num_tiles : gridDim.x / PAIR;  // a cluster has one tile
+  const int kb0 = SPL ? (int)((long long)p.num_kb * rank / splits) : 0;
+  const int kb1 = SPL ? (int)((long long)p.num_kb * (rank + 1) / splits) : p.num_kb;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < NACC; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 8 * PAIR);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&mapW);
+    prefetch_tmap(&mapX);
+  }
+  if (warp == 2) {
+    if constexpr (PAIR == 2) {
+      tmem_alloc_pair(tmem_slot, C::COLS);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, C::COLS);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR == 2) cluster_sync();  // the peer's barriers are initialised before use
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_launch_dependents();
+  griddep_wait();
+
+  // Tile order: blocks of eight w tiles walk the x tiles, so that the CTAs working at the same
+  // time share both operands in L2.
+  auto decode = [&](int tile, int* tm, int* tn) {
+    const int per = 8 * p.tiles_m, g = tile / per, r = tile - g * per;
+    const int gn = min(8, p.tiles_n - g * 8);
+    *tm = r / gn;
+    *tn = g * 8 + (r - *tm * gn);
+  };
+
+  if (warp == 0) {
+    // ---- producer
+    int s = 0;
+    uint32_t ph = 0, armed = 0, armed_ph = 0;
+    for (int t = unit0; t < p.num_tiles && !warp_abort(abort_flag); t += step) {
+      int tm, tn;
+      decode(t, &tm, &tn);
+      const int w_row = (tn * PAIR + (PAIR == 2 ? rank : 0)) * 128;
+      const int x_row = tm * BN + (PAIR == 2 ? rank * (BN / 2) : 0);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!warp_wait_bar(&empty[s], ph ^ 1, abort_flag)) break;
+        if (lane == 0) {
+          if (PAIR == 1 || rank == 0) {
+            mbar_arrive_expect_tx(&full[s], C::STAGE * PAIR);
+            armed |= 1u << s;
+            armed_ph = (armed_ph & ~(1u << s)) | (ph << s);
+          }
+          if constexpr (PAIR == 2) {
+            const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+            tma_load_2d_pair(&mapW, bar, sA + s * C::A_STAGE, kb * C::BK, w_row);
+            tma_load_2d_pair(&mapX, bar, sB + s * C::B_STAGE, kb * C::BK, x_row);
+          } else {
+            tma_load_2d(&mapW, &full[s], sA + s * C::A_STAGE, kb * C::BK, w_row);
+            tma_load_2d(&mapX, &full[s], sB + s * C::B_STAGE, kb * C::BK, x_row);
+          }
+        }
+        __syncwarp();
+        if (++s == STAGES) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    if (warp_abort(abort_flag) && lane == 0) {
+      // copies in flight land before the shared memory goes away
+      volatile int dummy = 0;
+      for (int i = 0; i < STAGES; ++i)
+        if (armed & (1u << i)) mbar_wait(&full[i], (armed_ph >> i) & 1, &dummy, kDrainNs);
+    }
+    __syncwarp();
+  } else if (warp == 1 && (PAIR == 1 || rank == 0)) {
+    // ---- MMA issuer (the pair's leader)
+    constexpr uint32_t idesc = make_idesc_16<T>(128 * PAIR, BN);
+    const uint64_t adesc = make_smem_desc(smem_u32(sA), 16, 1024, kSw128);
+    const uint64_t bdesc = make_smem_desc(smem_u32(sB), 16, 1024, kSw128);
+    int s = 0, it = 0;
+    uint32_t ph = 0;
+    bool issued = false;
+    for (int t = unit0; t < p.num_tiles && !warp_abort(abort_flag); t += step, ++it) {
+      const int b = it % NACC;
+      if (!warp_wait_bar(&tempty[b], ((it / NACC) & 1) ^ 1, abort_flag)) break;
+      tc_fence_after();
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!warp_wait_bar(&full[s], ph, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (lane == 0) {
+          const uint64_t a = adesc + ((s * C::A_STAGE) >> 4), x = bdesc + ((s * C::B_STAGE) >> 4);
+#pragma unroll
+          for (int j = 0; j < C::BK / 16; ++j) {
+            const uint32_t acc = kb != kb0 || j != 0 ? 1u : 0u;
+            if constexpr (PAIR == 2)
+              umma_f16_pair(tmem + b * BN, a + 2 * j, x + 2 * j, idesc, acc);
+            else
+              umma_f16(tmem + b * BN, a + 2 * j, x + 2 * j, idesc, acc);
+          }
+          if constexpr (PAIR == 2) {
+            umma_commit_pair(mapa_shared(smem_u32(&empty[s]), 0));
+            umma_commit_pair(mapa_shared(smem_u32(&empty[s]), 1));
+          } else {
+            umma_commit(&empty[s]);
+          }
+        }
+        __syncwarp();
+        issued = true;
+        if (++s == STAGES) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+      if (!ok) break;
+      if (lane == 0) {
+        if constexpr (PAIR == 2) {
+          umma_commit_pair(mapa_shared(smem_u32(&tfull[b]), 0));
+          umma_commit_pair(mapa_shared(smem_u32(&tfull[b]), 1));
+        } else {
+          umma_commit(&tfull[b]);
+        }
+      }
+      __syncwarp();
+    }
+    if (warp_abort(abort_flag) && issued && lane == 0) {
+      volatile int dummy = 0;
+      if constexpr (PAIR == 2)
+        umma_commit_pair(mapa_shared(smem_u32(drain), 0));
+      else
+        umma_commit(drain);
+      mbar_wait(drain, 0, &dummy, kDrainNs);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ---- epilogue: warp pairs share a TMEM lane quarter and alternate over its column chunks
+    constexpr int CW = 16;  // columns (rows of x) per step
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    int it = 0;
+    for (int t = unit0; t < p.num_tiles; t += step, ++it) {
+      int tm, tn;
+      decode(t, &tm, &tn);
+      const int n = (tn * PAIR + (PAIR == 2 ? rank : 0)) * 128 + quarter * 32 + lane;
+      const int m0 = tm * BN;
+      const float bias = !SPL && p.bias && n < p.n ? to_float(static_cast<const T*>(p.bias)[n]) : 0.0f;
+      const int b = it % NACC;
+      if (!__all_sync(0xffffffffu, mbar_wait_backoff(&tfull[b], (it / NACC) & 1, abort_flag, kTimeoutNs))) break;
+      tc_fence_after();
+      for (int c = half * CW; c < BN && m0 + c < p.m; c += 2 * CW) {
+        uint32_t r[CW];
+        tmem_ld_32x32b_x16(tmem + b * BN + c + ((uint32_t)(quarter * 32) << 16), r);
+        if constexpr (SPL) {
+          tmem_ld_wait();
+          float* part = reinterpret_cast<float*>(smem) + c * 128 + quarter * 32 + lane;
+#pragma unroll
+          for (int i = 0; i < CW; ++i) part[i * 128] = __uint_as_float(r[i]);
+        } else {
+          const int rows = min(CW, p.m - m0 - c);
+          T res[CW];
+          if (p.res && n < p.n) {
+            const T* src = static_cast<const T*>(p.res) + (long long)(m0 + c) * p.ldr + n;
+#pragma unroll
+            for (int i = 0; i < CW; ++i)
+              if (i < rows) res[i] = src[i * p.ldr];
+          }
+          tmem_ld_wait();
+          if (n < p.n) {
+            T* dst = static_cast<T*>(p.y) + (long long)(m0 + c) * p.ldy + n;
+#pragma unroll
+            for (int i = 0; i < CW; ++i) {
+              if (i >= rows) break;
+              float v = activate(__uint_as_float(r[i]) + bias, p.act);
+              if (p.res) v += to_float(res[i]);
+              dst[i * p.ldy] = round_to<T>(v);
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (PAIR == 2)
+          mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[b]), 0));
+        else
+          mbar_arrive(&tempty[b]);
+      }
+    }
+  }
+
+  if constexpr (SPL) {
+    // Partial tiles, [row of x][128 rows of w] in every CTA's shared memory, added in rank order;
+    // each CTA finishes its share of the rows of x.
+    __syncthreads();
+    cluster_sync();
+    int tm, tn;
+    decode(unit0, &tm, &tn);
+    const int rows = min(BN, p.m - tm * BN);
+    const int c0 = rows * (int)rank / (int)splits, c1 = rows * ((int)rank + 1) / (int)splits;
+    const uint32_t base = smem_u32(smem);
+    for (int i = c0 * 128 + threadIdx.x; i < c1 * 128; i += kTileThreads) {
+      const int n = tn * 128 + (i & 127), m = tm * BN + (i >> 7);
+      if (n >= p.n) continue;
+      float v = 0.0f;
+      for (uint32_t j = 0; j < splits; ++j) v += ld_cluster_f32(mapa_shared(base + i * 4, j));
+      if (p.bias) v += to_float(static_cast<const T*>(p.bias)[n]);
+      v = activate(v, p.act);
+      if (p.res) v += to_float(static_cast<const T*>(p.res)[m * p.ldr + n]);
+      static_cast<T*>(p.y)[m * p.ldy + n] = round_to<T>(v);
+    }
+    cluster_sync();  // the others have read this CTA's part
+  }
+  __syncthreads();
+  if constexpr (PAIR == 2) cluster_sync();  // no CTA leaves while its peer may use its memory
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.err, kLinearTimeout);
+  if (warp == 2) {
+    tc_fence_after();
+    if constexpr (PAIR == 2)
+      tmem_dealloc_pair(tmem, C::COLS);
+    else
+      tmem_dealloc(tmem, C::COLS);
+  }
+}
+
+// ------------------------------------------------------------------ host
+struct LinearPlan {
+  int bn = 0, pair = 1, split = 1;  // bn 0: linear_rows_kernel
+  bool copy_x = false, copy_w = false;
+  size_t x_bytes = 0, w_bytes = 0;
+};
+
+bool tma_rows(const void* p, long long ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
+
+LinearPlan linear_plan(const LinearParams& p, int sms) {
+  LinearPlan pl;
+  if (p.m <= kRowsMax) return pl;
+  const size_t pitch = ((size_t)p.k + 7) / 8 * 8 * 2;
+  pl.copy_x = !tma_rows(p.x, p.ldx);
+  pl.copy_w = !tma_rows(p.w, p.ldw);
+  pl.x_bytes = pl.copy_x ? (pitch * p.m + 255) / 256 * 256 : 0;
+  pl.w_bytes = pl.copy_w ? (pitch * p.n + 255) / 256 * 256 : 0;
+  const int kb = (p.k + 63) / 64, tn = (p.n + 127) / 128;
+  auto tiles = [&](int bn) { return (long long)((p.m + bn - 1) / bn) * tn; };
+  // CTA pairs of 256 x 256 where they fill the GPU; else the widest tile that fills it; else the
+  // narrowest one that holds the rows, with k split over a cluster
+  const long long pair_tiles = (long long)((p.m + 255) / 256) * ((p.n + 255) / 256);
+  if (pair_tiles * 2 >= sms) {
+    pl.bn = 256;
+    pl.pair = 2;
+    return pl;
+  }
+  pl.bn = p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
+  while (pl.split < 8 && tiles(pl.bn) * pl.split * 2 <= sms && kb >= pl.split * 2 * 4) pl.split *= 2;
+  return pl;
+}
+
+template <typename T, typename C>
+int launch_tiles(const LinearParams& p0, const LinearPlan& pl, const void* x, long long ldx, const void* w, long long ldw,
+                 int sms, cudaStream_t st) {
+  LinearParams p = p0;
+  p.num_kb = (p.k + 63) / 64;
+  p.tiles_m = (p.m + C::BN - 1) / C::BN;
+  p.tiles_n = (p.n + 128 * C::PAIR - 1) / (128 * C::PAIR);
+  const long long tiles = (long long)p.tiles_m * p.tiles_n;
+  SPINN_CHECK_ARG(tiles < (1ll << 30), "linear: too many tiles");
+  p.num_tiles = (int)tiles;
+  CUtensorMap mw, mx;
+  const bool half = std::is_same<T, __half>::value;
+  int rc = encode_tiled_2d_16(&mw, w, p.k, p.n, (uint64_t)ldw * 2, C::BK, 128, half);
+  if (rc) return rc;
+  rc = encode_tiled_2d_16(&mx, x, p.k, p.m, (uint64_t)ldx * 2, C::BK, C::BN / C::PAIR, half);
+  if (rc) return rc;
+  auto* kernel = linear_tile_kernel<T, C>;
+  SPINN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+  const int cluster = C::SPL ? pl.split : C::PAIR;
+  const int grid = C::SPL ? p.num_tiles * pl.split : std::min(p.num_tiles, sms / C::PAIR) * C::PAIR;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kTileThreads);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  SPINN_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, mw, mx, p));
+  return 0;
+}
+
+template <typename T>
+int linear_launch(const LinearParams& p, const LinearPlan& pl, void* ws, int sms, cudaStream_t st) {
+  if (pl.bn == 0) {
+    const dim3 grid((p.n + 15) / 16);
+    const int threads = kRowWarps * 32;
+    if (p.m <= 8)
+      return p.vec ? launch_dependent(linear_rows_kernel<T, 1, true>, grid, threads, 0, st, p)
+                   : launch_dependent(linear_rows_kernel<T, 1, false>, grid, threads, 0, st, p);
+    return p.vec ? launch_dependent(linear_rows_kernel<T, 2, true>, grid, threads, 0, st, p)
+                 : launch_dependent(linear_rows_kernel<T, 2, false>, grid, threads, 0, st, p);
+  }
+  const void *x = p.x, *w = p.w;
+  long long ldx = p.ldx, ldw = p.ldw;
+  if (pl.copy_x || pl.copy_w) {
+    PitchParams c = {};
+    c.k = p.k;
+    c.pitch = (p.k + 7) / 8 * 8;
+    if (pl.copy_x) {
+      c.src[0] = static_cast<const uint16_t*>(p.x);
+      c.dst[0] = static_cast<uint16_t*>(ws);
+      c.ld[0] = p.ldx;
+      c.rows[0] = p.m;
+      x = ws;
+      ldx = c.pitch;
+    }
+    if (pl.copy_w) {
+      c.src[1] = static_cast<const uint16_t*>(p.w);
+      c.dst[1] = reinterpret_cast<uint16_t*>(static_cast<char*>(ws) + pl.x_bytes);
+      c.ld[1] = p.ldw;
+      c.rows[1] = p.n;
+      w = c.dst[1];
+      ldw = c.pitch;
+    }
+    const int rc = launch_dependent(pitch_kernel, dim3(std::min(std::max(c.rows[0], c.rows[1]), sms * 8), 2), 256, 0, st, c);
+    if (rc) return rc;
+  }
+  if (pl.pair == 2) return launch_tiles<T, LinCfg<256, 2, false>>(p, pl, x, ldx, w, ldw, sms, st);
+  const bool spl = pl.split > 1;
+#define LINEAR_BN(W)                                                                        \
+  if (pl.bn == W)                                                                           \
+    return spl ? launch_tiles<T, LinCfg<W, 1, true>>(p, pl, x, ldx, w, ldw, sms, st)        \
+               : launch_tiles<T, LinCfg<W, 1, false>>(p, pl, x, ldx, w, ldw, sms, st);
+  LINEAR_BN(32)
+  LINEAR_BN(64)
+  LINEAR_BN(128)
+#undef LINEAR_BN
+  set_error("linear: no kernel for tile %d", pl.bn);
+  return SPINN_CUDA_EUNSUPPORTED;
+}
+
+int linear_params(const SpinnCudaLinear* l, LinearParams* p) {
+  SPINN_CHECK_ARG(l && l->x && l->w && l->y, "linear: x, w and y are required");
+  SPINN_CHECK_ARG(l->dtype == SPINN_CUDA_FP16 || l->dtype == SPINN_CUDA_BF16,
+                  "linear: element type %d not supported (fp16 or bf16; spinn_cuda_gemm takes fp32)", l->dtype);
+  SPINN_CHECK_ARG(l->m > 0 && l->n > 0 && l->k > 0, "linear: bad sizes %d x %d x %d", l->m, l->n, l->k);
+  SPINN_CHECK_ARG(l->x_stride >= l->k && l->w_stride >= l->k && l->y_stride >= l->n &&
+                      (!l->residual || l->residual_stride >= l->n),
+                  "linear: a row stride is shorter than its row");
+  SPINN_CHECK_ARG(l->act == 0 || l->act == 1 || l->act == 3 || l->act == SPINN_CUDA_ACT_GELU ||
+                      l->act == SPINN_CUDA_ACT_GELU_TANH,
+                  "linear: activation %d not supported", l->act);
+  SPINN_CHECK_ARG((((uintptr_t)l->x | (uintptr_t)l->w | (uintptr_t)l->y | (uintptr_t)l->bias | (uintptr_t)l->residual) & 1) == 0,
+                  "linear: misaligned pointer");
+  p->x = l->x;
+  p->w = l->w;
+  p->bias = l->bias;
+  p->res = l->residual;
+  p->y = l->y;
+  p->ldx = l->x_stride;
+  p->ldw = l->w_stride;
+  p->ldr = l->residual_stride;
+  p->ldy = l->y_stride;
+  p->m = l->m;
+  p->n = l->n;
+  p->k = l->k;
+  p->act = l->act;
+  p->vec = tma_rows(l->x, l->x_stride) && tma_rows(l->w, l->w_stride);
+  p->err = nullptr;
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+__attribute__((visibility("default"))) size_t spinn_cuda_linear_workspace(const SpinnCudaLinear* l) {
+  LinearParams p;
+  if (linear_params(l, &p)) return 0;
+  const LinearPlan pl = linear_plan(p, 148);  // the copies do not depend on the SM count
+  return pl.x_bytes + pl.w_bytes;
+}
+
+__attribute__((visibility("default"))) int spinn_cuda_linear(const SpinnCudaLinear* l, void* workspace,
+                                                             size_t workspace_bytes, void* stream) {
+  LinearParams p;
+  int rc = linear_params(l, &p);
+  if (rc) return rc;
+  int dev;
+  rc = check_stream_device("linear", stream, &dev);
+  if (rc) return rc;
+  const int sms = sm_count(dev);
+  const LinearPlan pl = linear_plan(p, sms);
+  const size_t need = pl.x_bytes + pl.w_bytes;
+  SPINN_CHECK_ARG(!need || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+                  "linear: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
+  rc = decode_error_word(dev, &p.err);
+  if (rc) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return l->dtype == SPINN_CUDA_FP16 ? linear_launch<__half>(p, pl, workspace, sms, st)
+                                     : linear_launch<__nv_bfloat16>(p, pl, workspace, sms, st);
+}
+
+}  // extern "C"
+}  // namespace spinn

@@ -82,6 +82,33 @@ int encode_tiled_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t
   return 0;
 }
 
+int encode_tiled_2d_16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
+                       uint32_t box_inner, uint32_t box_outer, bool fp16) {
+  std::call_once(g_once, load_entry_points);
+  if (!g_tiled) {
+    set_error("cuTensorMapEncodeTiled unavailable from the driver");
+    return SPINN_CUDA_ECUDA;
+  }
+  SPINN_CHECK_ARG((reinterpret_cast<uintptr_t>(base) & 15) == 0 && row_stride_bytes % 16 == 0,
+                  "tensor map base %p or row stride %llu not a multiple of 16", base,
+                  (unsigned long long)row_stride_bytes);
+  cuuint64_t dims[2] = {inner, outer};
+  cuuint64_t strides[1] = {row_stride_bytes};
+  cuuint32_t box[2] = {box_inner, box_outer};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = g_tiled(map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                       const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled (16-bit) failed (%d): dims %llu x %llu stride %llu", (int)r,
+              (unsigned long long)inner, (unsigned long long)outer, (unsigned long long)row_stride_bytes);
+    return SPINN_CUDA_ECUDA;
+  }
+  small_tensor_fixup(map, row_stride_bytes * outer);
+  return 0;
+}
+
 int encode_tiled_3d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t planes,
                     uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle) {
   std::call_once(g_once, load_entry_points);

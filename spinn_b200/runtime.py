@@ -5,8 +5,8 @@
   parameter blocks; ``SPINN/run_time/ops/conv/conv2d.c``, ``ops/mm/gemm.c``,
   ``ops/mm/matmul.c``).  Arrays may be NumPy (host memory, like the reference arena) or
   CUDA torch tensors (device memory).
-* Decoder serving -- :func:`cache_append`, :func:`paged_attention`, :func:`cache_evict` work on
-  CUDA torch tensors in place, on torch's current stream of their device; :func:`stream_sync`
+* Decoder serving -- :func:`linear`, :func:`cache_append`, :func:`paged_attention`, :func:`cache_evict` work on
+  CUDA torch tensors, on torch's current stream of their device; :func:`stream_sync`
   reports what only the device could see (a bad page number, a length beyond its table).
 * Model level -- :class:`Model` wraps ``spinn_cuda_load / _plan / _run / _free``, the
   device-resident counterpart of ``spinn_load / spinn_plan / spinn_run / spinn_free``
@@ -121,6 +121,8 @@ _TABLE = struct.Struct("<QQqii")               # SpinnCudaPageTable
 _APPEND = struct.Struct("<QQqqqqQii")          # SpinnCudaAppend
 _ATTENTION = struct.Struct("<QQqqqqQQqqqqiifi")  # SpinnCudaAttention
 _EVICT = struct.Struct("<QQqqqqQqiiQQii")      # SpinnCudaEvict
+_LINEAR = struct.Struct("<QQQQQqqqqiiiiii")    # SpinnCudaLinear
+_ACTS = {"none": 0, "relu": 1, "silu": 3, "gelu": 6, "gelu_tanh": 7}
 _torch = None
 _dtype_codes: dict = {}
 
@@ -204,6 +206,55 @@ def stream_sync(device: Optional[int] = None) -> None:
     torch = _torch_module()
     _queue(torch.cuda.current_device() if device is None else device,
            lambda st: check(lib().spinn_cuda_stream_sync(st), "spinn_cuda_stream_sync"))
+
+
+def linear(x, w, y, bias=None, residual=None, act: str = "none") -> None:
+    """``y = act(x @ w.T + bias) + residual`` in fp16 or bf16 (fp32: :func:`gemm`), accumulated in fp32
+    and rounded once.
+
+    ``x`` is ``[m, k]``, ``w`` ``[n, k]``, ``y`` and ``residual`` ``[m, n]``, with contiguous rows of any
+    stride, ``bias`` ``[n]``; ``act`` is "none", "relu", "silu", "gelu" (by erf) or "gelu_tanh".  ``y``
+    may be ``residual`` itself.  Rows of ``x`` and ``w`` that start on 16-byte boundaries are read in
+    place; others are copied first when ``x`` has more than 16 rows."""
+    torch = _torch_module()
+    name = "linear"
+    dev = _on_device(name, x, w, y, bias, residual)
+    code = _dtype_codes.get(x.dtype)
+    if x.dtype != w.dtype or x.dtype != y.dtype or code not in (_L.FP16, _L.BF16):
+        raise TypeError(f"{name}: x, w and y must all be float16 or all bfloat16")
+    if x.dim() != 2 or w.dim() != 2 or y.dim() != 2:
+        raise ValueError(f"{name}: x, w and y must be 2-D")
+    (m, k), (n, k2) = x.shape, w.shape
+    if k != k2 or y.shape[0] != m or y.shape[1] != n:
+        raise ValueError(f"{name}: shapes {tuple(x.shape)}, {tuple(w.shape)} and {tuple(y.shape)} do not match")
+    xs, ws, ys, rs = x.stride(), w.stride(), y.stride(), (n, 1)
+    bp = rp = 0
+    if bias is not None:
+        if bias.dtype != x.dtype or tuple(bias.shape) != (n,) or (bias.stride(0) != 1 and n != 1):
+            raise ValueError(f"{name}: bias must be a contiguous [{n}] of {x.dtype}")
+        bp = bias.data_ptr()
+    if residual is not None:
+        if residual.dtype != x.dtype or residual.shape != y.shape:
+            raise ValueError(f"{name}: residual must be {tuple(y.shape)} of {x.dtype}")
+        rs = residual.stride()
+        rp = residual.data_ptr()
+    if act not in _ACTS:
+        raise ValueError(f"{name}: act must be one of {', '.join(_ACTS)}")
+    if (xs[1] != 1 and k != 1) or (ws[1] != 1 and k != 1) or (n != 1 and (ys[1] != 1 or rs[1] != 1)):
+        raise ValueError(f"{name}: rows must be contiguous")
+    if m == 0:
+        return
+    # the stride of a single row means nothing
+    desc = _LINEAR.pack(x.data_ptr(), w.data_ptr(), bp, rp, y.data_ptr(), xs[0] if m > 1 else k, ws[0] if n > 1 else k,
+                        rs[0] if m > 1 else n, ys[0] if m > 1 else n, m, n, k, code, _ACTS[act], 0)
+
+    def call(st):
+        L = lib()
+        size = L.spinn_cuda_linear_workspace(desc)
+        space = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        check(L.spinn_cuda_linear(desc, space.data_ptr() if size else None, size, st), "spinn_cuda_linear")
+
+    _queue(dev, call)
 
 
 def cache_append(k, v, k_cache, v_cache, page_table, lens, starts=None) -> None:

@@ -185,3 +185,40 @@ def test_attention_shares_cover_the_work_once():
             a, b = starts[out[2]]
             assert a <= u < b
     assert L.spinn_cuda_diag_attention_share(0, 1, 0, 0, out) == lib.EINVAL
+
+
+# ------------------------------------------------------------------ linear
+def linear(**kw):
+    f = dict(x=P, w=P, b=0, r=0, y=P, ldx=64, ldw=64, ldr=0, ldy=32, m=4, n=32, k=64, dtype=lib.BF16, act=0)
+    f.update(kw)
+    return runtime._LINEAR.pack(f["x"], f["w"], f["b"], f["r"], f["y"], f["ldx"], f["ldw"], f["ldr"], f["ldy"], f["m"],
+                                f["n"], f["k"], f["dtype"], f["act"], 0)
+
+
+@pytest.mark.parametrize("kw,match", [(dict(x=0), "required"), (dict(w=0), "required"), (dict(y=0), "required"),
+                                      (dict(dtype=lib.FP32), "type 1"), (dict(m=0), "sizes"), (dict(n=-1), "sizes"),
+                                      (dict(k=0), "sizes"), (dict(ldx=63), "stride"), (dict(ldw=0), "stride"),
+                                      (dict(ldy=31), "stride"), (dict(r=P, ldr=8), "stride"), (dict(act=4), "activation"),
+                                      (dict(act=2), "activation"), (dict(w=P + 1), "misaligned"),
+                                      (dict(b=P + 1), "misaligned")])
+def test_linear_refusals(kw, match):
+    refused("spinn_cuda_linear", linear(**kw), None, 0, None, match=match)
+    assert lib.lib().spinn_cuda_linear_workspace(linear(**kw)) == 0
+
+
+def test_linear_workspace_holds_the_rows_that_are_off_alignment():
+    ws = lib.lib().spinn_cuda_linear_workspace
+    assert ws(linear(m=17)) == 0                              # aligned rows are read in place
+    assert ws(linear(m=16, k=63, ldx=63, ldw=63)) == 0        # few rows: any alignment
+    up = lambda b: -(-b // 256) * 256                         # noqa: E731
+    assert ws(linear(m=17, k=63, ldx=63)) == up(17 * 128)
+    assert ws(linear(m=17, k=63, ldx=64, ldw=63)) == up(32 * 128)
+    assert ws(linear(m=17, x=P + 2)) == up(17 * 128)
+    assert ws(linear(m=2 ** 20, n=2 ** 20, k=8191, ldx=8191, ldw=8191, ldy=2 ** 20)) == 2 * 2 ** 20 * 16384  # past 32 bits
+
+
+def test_python_linear_refuses_what_does_not_match():
+    torch = pytest.importorskip("torch")
+    x = torch.zeros(2, 8, dtype=torch.float16)
+    with pytest.raises(TypeError, match="CUDA"):
+        runtime.linear(x, x, torch.zeros(2, 2, dtype=torch.float16))

@@ -1,0 +1,146 @@
+"""16-bit linear layers on the GPU against the same formula in 64 bits."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def rt(cuda_lib):
+    from spinn_b200 import runtime
+    return runtime
+
+
+def act64(z, act):
+    if act == "relu":
+        return z.clamp_min(0)
+    if act == "silu":
+        return z * torch.sigmoid(z)
+    if act == "gelu":
+        return 0.5 * z * (1 + torch.erf(z / math.sqrt(2)))
+    if act == "gelu_tanh":
+        return 0.5 * z * (1 + torch.tanh(math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)))
+    return z
+
+
+def rows(shape, dtype, pad=0, shift=0, scale=1.0):
+    """A matrix whose rows are `pad` elements apart beyond their length, `shift` elements into its
+    storage; the gaps hold NaN."""
+    m, k = shape
+    flat = torch.full((m * (k + pad) + shift + 8,), float("nan"), dtype=dtype, device="cuda")
+    t = flat[shift:shift + m * (k + pad)].view(m, k + pad)[:, :k]
+    t.copy_((torch.randn(m, k, device="cuda") * scale).to(dtype))
+    return t
+
+
+CASES = [
+    # dtype, m, k, n, act, bias, residual, (pad, shift) of x, w, y, residual
+    ("fp16", 1, 1, 1, "none", False, False, (0, 0)),
+    ("bf16", 1, 64, 16, "none", True, True, (0, 0)),
+    ("fp16", 1, 2048, 1000, "none", True, False, (0, 0)),
+    ("bf16", 3, 1001, 77, "gelu", True, True, (0, 0)),      # odd rows: element loads
+    ("bf16", 8, 520, 100, "silu", True, False, (8, 8)),
+    ("fp16", 9, 520, 100, "gelu_tanh", False, True, (3, 1)),
+    ("bf16", 16, 4096, 48, "relu", True, True, (0, 0)),
+    ("fp16", 16, 31, 5, "silu", True, True, (1, 1)),
+    ("bf16", 17, 64, 128, "none", False, False, (0, 0)),    # first size of the tile kernel
+    ("fp16", 17, 1, 1, "gelu", True, True, (0, 0)),
+    ("bf16", 32, 40, 130, "silu", True, True, (0, 0)),
+    ("bf16", 48, 4096, 512, "none", True, True, (0, 0)),    # k split over a cluster
+    ("fp16", 33, 1000, 257, "gelu", True, True, (0, 0)),
+    ("bf16", 64, 2048, 1000, "relu", False, True, (8, 16)),
+    ("fp16", 65, 513, 129, "gelu_tanh", True, True, (0, 0)),  # operands copied to an aligned pitch
+    ("bf16", 100, 777, 333, "none", True, True, (5, 3)),
+    ("bf16", 128, 128, 128, "silu", False, False, (0, 0)),
+    ("fp16", 129, 200, 64, "relu", True, True, (0, 0)),
+    ("bf16", 777, 1001, 2047, "gelu", True, True, (0, 0)),
+    ("fp16", 300, 4096, 130, "none", False, True, (0, 0)),
+    ("bf16", 2100, 320, 2300, "silu", True, True, (0, 0)),  # CTA pairs, ragged on both sides
+    ("fp16", 2048, 2048, 2304, "none", False, False, (0, 0)),
+    ("bf16", 5000, 64, 1100, "gelu_tanh", True, True, (1, 1)),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: f"{c[0]}-{c[1]}x{c[2]}x{c[3]}-{c[4]}-{c[7][0]}.{c[7][1]}")
+def test_linear_matches_its_definition(rt, case):
+    dtype, m, k, n, act, has_bias, has_res, (pad, shift) = case
+    torch.manual_seed(m * 7 + k * 3 + n)
+    dt = DTYPES[dtype]
+    x, w = rows((m, k), dt, pad, shift), rows((n, k), dt, pad, shift, k ** -0.5)
+    y, res = rows((m, n), dt, pad, shift), rows((m, n), dt, pad, shift) if has_res else None
+    bias = torch.randn(n, device="cuda").to(dt) if has_bias else None
+    gaps = y.as_strided((m, n + pad), (n + pad, 1), y.storage_offset())[:, n:].clone()
+    rt.linear(x, w, y, bias, res, act)
+    rt.stream_sync()
+    z = x.double() @ w.double().T
+    mass = x.double().abs() @ w.double().abs().T
+    if has_bias:
+        z = z + bias.double()
+    want = act64(z, act)
+    if has_res:
+        want = want + res.double()
+    # the sum of k exact products in fp32, in any order, the tensor core's truncating adder counted
+    # as a whole step: k 2^-23 of the sum of their magnitudes; no activation is steeper than 1.13;
+    # its own arithmetic is good to 2^-20 of |z| + 1; then fp32 adds and one rounding
+    half = torch.finfo(dt).eps / 2
+    slack = 1.13 * k * 2.0 ** -23 * mass + (0 if act == "none" else 2.0 ** -20) * (z.abs() + 1) + 2.0 ** -22 * (
+        z.abs() + want.abs())
+    tiny = 2.0 ** -25 if dtype == "fp16" else 0.0  # fp16 rounds in steps of 2^-24 below 2^-14
+    tol = half * want.abs() + (1 + half) * slack + tiny
+    err = (y.double() - want).abs()
+    assert torch.isfinite(y).all()
+    assert (err <= tol).all(), float((err / tol.clamp_min(1e-30)).max())
+    after = y.as_strided((m, n + pad), (n + pad, 1), y.storage_offset())[:, n:]
+    assert torch.equal(torch.isnan(after), torch.isnan(gaps))
+
+
+def test_linear_in_place_of_its_residual(rt):
+    for m in (5, 50, 700):
+        x = rows((m, 256), torch.bfloat16)
+        w = rows((384, 256), torch.bfloat16, scale=1 / 16)
+        r = rows((m, 384), torch.bfloat16)
+        y = torch.empty_like(r)
+        rt.linear(x, w, y, None, r)
+        rt.linear(x, w, r, None, r)
+        rt.stream_sync()
+        assert torch.equal(y, r)
+
+
+def test_linear_extreme_activations(rt):
+    """Large and infinite pre-activations: the activations' limits, no NaN from inf - inf."""
+    eye = torch.eye(16, device="cuda", dtype=torch.bfloat16)
+    vals = torch.tensor([0.0, -0.0, 1.0, -1.0, 30.0, -30.0, 90.0, -90.0, 3e4, -3e4, 1e30, -1e30, 3e38, -3e38, 1e-30, -5.0],
+                        device="cuda", dtype=torch.bfloat16)
+    for m in (1, 40):
+        x = vals.expand(m, 16).contiguous()
+        for act in ("none", "relu", "silu", "gelu", "gelu_tanh"):
+            y = torch.empty(m, 16, device="cuda", dtype=torch.bfloat16)
+            rt.linear(x, eye, y, act=act)
+            rt.stream_sync()
+            want = act64(x.double(), act)
+            # an infinite cube in 64 bits never occurs; bf16 keeps 8 bits
+            tol = 2.0 ** -8 * want.abs() + 2.0 ** -20
+            assert ((y.double() - want).abs() <= tol).all(), (act, m, y[0], want[0])
+
+
+def test_linear_captured_and_replayed(rt):
+    x, w = rows((77, 333), torch.float16), rows((200, 333), torch.float16, scale=0.05)  # with copies
+    y, y2 = rows((77, 200), torch.float16), rows((77, 200), torch.float16)
+    rt.linear(x, w, y, act="silu")
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        rt.linear(x, w, y2, act="silu")
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, y2)
+    x.mul_(-1)
+    rt.linear(x, w, y, act="silu")
+    graph.replay()
+    rt.stream_sync()
+    assert torch.equal(y, y2)
