@@ -1,4 +1,5 @@
-"""Builds libspinn_cuda.so in-tree with nvcc for sm_100a.
+"""Builds libspinn_cuda.so in-tree with nvcc for sm_100a, and the torch binding of its
+decoder-serving operators (_torch_ops.so) with the host compiler.
 
 Usage: ``python -m spinn_b200.build [--force] [--verbose]``.  Object files go to
 ``spinn_b200/_build/`` and the shared library to ``spinn_b200/libspinn_cuda.so``; both are
@@ -8,10 +9,12 @@ under ``csrc/`` or ``include/`` is newer than its object.
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -19,6 +22,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libspinn_cuda.so")
+TORCH_OPS = os.path.join(HERE, "_torch_ops.so")
 SOURCES = ["tmap.cpp", "tc_gemm.cu", "glue.cu", "runtime.cpp", "abi.cpp", "noalloc.cu", "winograd.cu", "tail.cu",
            "cache.cu", "attention.cu", "attention_fp16.cu", "attention_bf16.cu", "attention_fp32.cu",
            "linear.cu"]
@@ -70,6 +74,35 @@ def _compile(src: str, force: bool, verbose: bool, extra: list) -> str:
     return obj
 
 
+def _build_torch_ops(force: bool, verbose: bool) -> str:
+    """csrc/torch_ops.cpp against the installed torch; rebuilt when it, the C header or torch's
+    version changes."""
+    import importlib.metadata
+    src = os.path.join(CSRC, "torch_ops.cpp")
+    stamp = os.path.join(BUILD, "torch_ops.version")
+    version = importlib.metadata.version("torch")
+    newest = max(os.path.getmtime(src), _headers_mtime())
+    if not force and os.path.exists(TORCH_OPS) and os.path.exists(stamp) and \
+            os.path.getmtime(TORCH_OPS) >= newest and open(stamp).read() == version:
+        return TORCH_OPS
+    root = os.path.join(os.path.dirname(importlib.util.find_spec("torch").origin))
+    cxx = host_compiler()[-1] if host_compiler() else "g++"
+    cmd = [cxx, "-O2", "-std=c++20", "-fPIC", "-shared", "-fvisibility=hidden", "-I" + os.path.join(root, "include"),
+           "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-I" + os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include"),
+           "-I" + sysconfig.get_paths()["include"], src, "-o", TORCH_OPS, "-L" + HERE, "-l:libspinn_cuda.so",
+           "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+           "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cxx} failed on torch_ops.cpp:\n{r.stdout}\n{r.stderr}")
+    with open(stamp, "w") as f:
+        f.write(version)
+    return TORCH_OPS
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     extra = ["-Xptxas", "-v"] if ptxas_verbose else []
@@ -83,6 +116,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    _build_torch_ops(force, verbose)
     return LIB
 
 

@@ -116,96 +116,33 @@ def matmul(a, b, y) -> None:
 
 
 # ------------------------------------------------------------------ decoder serving
-_CACHE = struct.Struct("<QQqqqiiiiii")         # SpinnCudaCache
-_TABLE = struct.Struct("<QQqii")               # SpinnCudaPageTable
-_APPEND = struct.Struct("<QQqqqqQii")          # SpinnCudaAppend
-_ATTENTION = struct.Struct("<QQqqqqQQqqqqiifi")  # SpinnCudaAttention
-_EVICT = struct.Struct("<QQqqqqQqiiQQii")      # SpinnCudaEvict
-_LINEAR = struct.Struct("<QQQQQqqqqiiiiii")    # SpinnCudaLinear
+# The calls are taken apart by the native binding (csrc/torch_ops.cpp): a decoding step makes many
+# of a few microseconds each.
 _ACTS = {"none": 0, "relu": 1, "silu": 3, "gelu": 6, "gelu_tanh": 7}
-_torch = None
-_dtype_codes: dict = {}
+_binding = None
 
 
-def _torch_module():
-    global _torch
-    if _torch is None:
-        import torch
-        _dtype_codes.update({torch.float32: _L.FP32, torch.float16: _L.FP16, torch.bfloat16: _L.BF16})
-        _torch = torch
-    return _torch
-
-
-def _on_device(name, *tensors) -> int:
-    """The one CUDA device of the tensors (None among them is skipped)."""
-    dev = tensors[0].get_device()
-    if dev < 0:
-        raise TypeError(f"{name}: CUDA tensors are required")
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"{name}: tensors on different devices")
-    return dev
-
-
-def _queue(dev: int, call) -> None:
-    """``call(stream)`` with `dev` as the current device and torch's current stream of it."""
-    torch = _torch
-    if torch.cuda.current_device() == dev:
-        call(torch.cuda.current_stream(dev).cuda_stream)
-    else:
-        with torch.cuda.device(dev):
-            call(torch.cuda.current_stream(dev).cuda_stream)
-
-
-def _cache_desc(name, k, v) -> bytes:
-    if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype:
-        raise ValueError(f"{name}: k_cache and v_cache must be [pages, page_size, heads, dim] of one shape, "
-                         "layout and type")
-    code = _dtype_codes.get(k.dtype)
-    if code is None:
-        raise TypeError(f"{name}: caches of {k.dtype} are not supported (float32, float16, bfloat16)")
-    pages, page, heads, dim = k.shape
-    ps, ts, hs, es = k.stride()
-    if es != 1 and dim != 1:
-        raise ValueError(f"{name}: the cache's last dimension must be contiguous")
-    return _CACHE.pack(k.data_ptr(), v.data_ptr(), ps, ts, hs, code, pages, page, heads, dim, 0)
-
-
-def _table_desc(name, table, lens) -> bytes:
-    i32 = _torch.int32
-    if table.dtype != i32 or lens.dtype != i32:
-        raise TypeError(f"{name}: page_table and lens must be int32")
-    if table.dim() != 2 or lens.dim() != 1 or lens.shape[0] != table.shape[0] or not lens.is_contiguous() or \
-            (table.stride(1) != 1 and table.shape[1] != 1):
-        raise ValueError(f"{name}: page_table must be [seqs, max_pages] with contiguous rows, lens [seqs]")
-    return _TABLE.pack(table.data_ptr(), lens.data_ptr(), table.stride(0), table.shape[0], table.shape[1])
-
-
-def _rows(name, what, t, cache, shape):
-    """(pointer, stride, stride) of a [n, heads, dim] tensor of the cache's type."""
-    if t.dtype != cache.dtype:
-        raise TypeError(f"{name}: {what} must have the cache's type {cache.dtype}, not {t.dtype}")
-    if tuple(t.shape) != shape or (t.stride(2) != 1 and shape[2] != 1):
-        raise ValueError(f"{name}: {what} must be {shape} with contiguous rows, not {tuple(t.shape)}")
-    return t.data_ptr(), t.stride(0), t.stride(1)
-
-
-def _weights(name, what, t, seqs, heads):
-    if t is None:
-        return 0, 0, 0
-    if t.dtype != _torch.float32:
-        raise TypeError(f"{name}: {what} must be float32")
-    if t.dim() != 3 or t.shape[0] != seqs or t.shape[1] != heads or (t.stride(2) != 1 and t.shape[2] != 1):
-        raise ValueError(f"{name}: {what} must be [{seqs}, {heads}, length] with contiguous rows")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+def _ops():
+    """The torch binding, loaded once (raises if it is absent: there is no fallback)."""
+    global _binding
+    if _binding is None:
+        import torch  # noqa: F401  (the binding links against it)
+        lib()
+        try:
+            from . import _torch_ops
+        except ImportError as e:
+            raise ImportError("spinn_b200/_torch_ops.so does not load; build it with "
+                              f"`python -m spinn_b200.build` ({e})") from e
+        _binding = _torch_ops
+    return _binding
 
 
 def stream_sync(device: Optional[int] = None) -> None:
     """Waits for torch's current stream and raises the deferred error of the operators below, if
     any (``spinn_cuda_stream_sync``).  Not during graph capture."""
-    torch = _torch_module()
-    _queue(torch.cuda.current_device() if device is None else device,
-           lambda st: check(lib().spinn_cuda_stream_sync(st), "spinn_cuda_stream_sync"))
+    import torch
+    with torch.cuda.device(device):
+        check(lib().spinn_cuda_stream_sync(torch.cuda.current_stream().cuda_stream), "spinn_cuda_stream_sync")
 
 
 def linear(x, w, y, bias=None, residual=None, act: str = "none") -> None:
@@ -216,45 +153,10 @@ def linear(x, w, y, bias=None, residual=None, act: str = "none") -> None:
     stride, ``bias`` ``[n]``; ``act`` is "none", "relu", "silu", "gelu" (by erf) or "gelu_tanh".  ``y``
     may be ``residual`` itself.  Rows of ``x`` and ``w`` that start on 16-byte boundaries are read in
     place; others are copied first when ``x`` has more than 16 rows."""
-    torch = _torch_module()
-    name = "linear"
-    dev = _on_device(name, x, w, y, bias, residual)
-    code = _dtype_codes.get(x.dtype)
-    if x.dtype != w.dtype or x.dtype != y.dtype or code not in (_L.FP16, _L.BF16):
-        raise TypeError(f"{name}: x, w and y must all be float16 or all bfloat16")
-    if x.dim() != 2 or w.dim() != 2 or y.dim() != 2:
-        raise ValueError(f"{name}: x, w and y must be 2-D")
-    (m, k), (n, k2) = x.shape, w.shape
-    if k != k2 or y.shape[0] != m or y.shape[1] != n:
-        raise ValueError(f"{name}: shapes {tuple(x.shape)}, {tuple(w.shape)} and {tuple(y.shape)} do not match")
-    xs, ws, ys, rs = x.stride(), w.stride(), y.stride(), (n, 1)
-    bp = rp = 0
-    if bias is not None:
-        if bias.dtype != x.dtype or tuple(bias.shape) != (n,) or (bias.stride(0) != 1 and n != 1):
-            raise ValueError(f"{name}: bias must be a contiguous [{n}] of {x.dtype}")
-        bp = bias.data_ptr()
-    if residual is not None:
-        if residual.dtype != x.dtype or residual.shape != y.shape:
-            raise ValueError(f"{name}: residual must be {tuple(y.shape)} of {x.dtype}")
-        rs = residual.stride()
-        rp = residual.data_ptr()
-    if act not in _ACTS:
-        raise ValueError(f"{name}: act must be one of {', '.join(_ACTS)}")
-    if (xs[1] != 1 and k != 1) or (ws[1] != 1 and k != 1) or (n != 1 and (ys[1] != 1 or rs[1] != 1)):
-        raise ValueError(f"{name}: rows must be contiguous")
-    if m == 0:
-        return
-    # the stride of a single row means nothing
-    desc = _LINEAR.pack(x.data_ptr(), w.data_ptr(), bp, rp, y.data_ptr(), xs[0] if m > 1 else k, ws[0] if n > 1 else k,
-                        rs[0] if m > 1 else n, ys[0] if m > 1 else n, m, n, k, code, _ACTS[act], 0)
-
-    def call(st):
-        L = lib()
-        size = L.spinn_cuda_linear_workspace(desc)
-        space = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-        check(L.spinn_cuda_linear(desc, space.data_ptr() if size else None, size, st), "spinn_cuda_linear")
-
-    _queue(dev, call)
+    code = _ACTS.get(act)
+    if code is None:
+        raise ValueError(f"linear: act must be one of {', '.join(_ACTS)}")
+    (_binding or _ops()).linear(x, w, y, bias, residual, code)
 
 
 def cache_append(k, v, k_cache, v_cache, page_table, lens, starts=None) -> None:
@@ -265,27 +167,7 @@ def cache_append(k, v, k_cache, v_cache, page_table, lens, starts=None) -> None:
     ``lens`` (the lengths before) is not changed.  Caches are ``[pages, page_size, kv_heads,
     head_dim]`` in fp32, fp16 or bf16 with any strides but a contiguous last dimension,
     ``page_table`` is int32 ``[seqs, max_pages]``."""
-    torch = _torch_module()
-    name = "cache_append"
-    dev = _on_device(name, k_cache, v_cache, k, v, page_table, lens, starts)
-    cache, table = _cache_desc(name, k_cache, v_cache), _table_desc(name, page_table, lens)
-    tokens = k.shape[0]
-    shape = (tokens, k_cache.shape[2], k_cache.shape[3])
-    kp, kt, kh = _rows(name, "k", k, k_cache, shape)
-    vp, vt, vh = _rows(name, "v", v, k_cache, shape)
-    sp = 0
-    if starts is not None:
-        if starts.dtype != torch.int32:
-            raise TypeError(f"{name}: starts must be int32")
-        if starts.dim() != 1 or starts.shape[0] != lens.shape[0] + 1 or not starts.is_contiguous():
-            raise ValueError(f"{name}: starts must be [seqs + 1]")
-        sp = starts.data_ptr()
-    elif tokens != lens.shape[0]:
-        raise ValueError(f"{name}: {tokens} rows for {lens.shape[0]} sequences without starts")
-    if tokens == 0:
-        return
-    rows = _APPEND.pack(kp, vp, kt, kh, vt, vh, sp, tokens, 0)
-    _queue(dev, lambda st: check(lib().spinn_cuda_cache_append(cache, table, rows, st), "spinn_cuda_cache_append"))
+    (_binding or _ops()).cache_append(k, v, k_cache, v_cache, page_table, lens, starts)
 
 
 def paged_attention(q, k_cache, v_cache, page_table, lens, y, scale=None, weights=None, weights_out=None) -> None:
@@ -296,37 +178,7 @@ def paged_attention(q, k_cache, v_cache, page_table, lens, y, scale=None, weight
     length 0 gets zeros.  With ``weights_out`` (fp32 ``[seqs, kv_heads, length]``) the probabilities
     of each key head's queries are summed and added to ``weights`` (zeros when None; may be
     ``weights_out`` itself); entries past a sequence's length are left as they were."""
-    torch = _torch_module()
-    name = "paged_attention"
-    if lens.numel() == 0:
-        return
-    dev = _on_device(name, k_cache, v_cache, q, page_table, lens, y, weights, weights_out)
-    cache, table = _cache_desc(name, k_cache, v_cache), _table_desc(name, page_table, lens)
-    seqs, heads, dim = lens.shape[0], k_cache.shape[2], k_cache.shape[3]
-    if q.dim() != 3:
-        raise ValueError(f"{name}: q must be [seqs, q_heads, head_dim]")
-    q_heads = q.shape[1]
-    qp, qs, qh = _rows(name, "q", q, k_cache, (seqs, q_heads, dim))
-    yp, ys, yh = _rows(name, "y", y, k_cache, (seqs, q_heads, dim))
-    wp, ws, wh = _weights(name, "weights", weights, seqs, heads)
-    op, os_, oh = _weights(name, "weights_out", weights_out, seqs, heads)
-    capacity = 0
-    if weights_out is not None:
-        capacity = weights_out.shape[2]
-        if weights is not None:
-            capacity = min(capacity, weights.shape[2])
-    elif weights is not None:
-        raise ValueError(f"{name}: weights without weights_out")
-    desc = _ATTENTION.pack(qp, yp, qs, qh, ys, yh, wp, op, ws, wh, os_, oh, capacity, q_heads,
-                           dim ** -0.5 if scale is None else scale, 0)
-
-    def call(st):
-        L = lib()
-        size = L.spinn_cuda_paged_attention_workspace(cache, table, desc)
-        space = torch.empty(size, dtype=torch.uint8, device=q.device)
-        check(L.spinn_cuda_paged_attention(cache, table, desc, space.data_ptr(), size, st), "spinn_cuda_paged_attention")
-
-    _queue(dev, call)
+    (_binding or _ops()).paged_attention(q, k_cache, v_cache, page_table, lens, y, scale, weights, weights_out)
 
 
 def cache_evict(k_cache, v_cache, page_table, lens, weights, weights_out, out_table, new_lens, kept, budget,
@@ -340,28 +192,8 @@ def cache_evict(k_cache, v_cache, page_table, lens, weights, weights_out, out_ta
     reads.  ``new_lens`` (int32 ``[seqs]``) gets the new lengths, ``kept`` (int32 ``[seqs, kv_heads,
     budget]``) the slots that were kept (-1 past the new length), ``weights_out`` their weights and
     zeros from there to the old length; it may be ``weights`` itself."""
-    torch = _torch_module()
-    name = "cache_evict"
-    if lens.numel() == 0:
-        return
-    dev = _on_device(name, k_cache, v_cache, page_table, lens, weights, weights_out, out_table, new_lens, kept)
-    cache, table = _cache_desc(name, k_cache, v_cache), _table_desc(name, page_table, lens)
-    seqs, heads = lens.shape[0], k_cache.shape[2]
-    i32 = torch.int32
-    if out_table.dtype != i32 or new_lens.dtype != i32 or kept.dtype != i32:
-        raise TypeError(f"{name}: out_table, new_lens and kept must be int32")
-    if out_table.dim() != 2 or out_table.shape[0] != seqs or (out_table.stride(1) != 1 and out_table.shape[1] != 1):
-        raise ValueError(f"{name}: out_table must be [seqs, max_pages] with contiguous rows")
-    if new_lens.shape != lens.shape or not new_lens.is_contiguous():
-        raise ValueError(f"{name}: new_lens must be [seqs]")
-    if tuple(kept.shape) != (seqs, heads, budget) or not kept.is_contiguous():
-        raise ValueError(f"{name}: kept must be [{seqs}, {heads}, {budget}], contiguous")
-    wp, ws, wh = _weights(name, "weights", weights, seqs, heads)
-    op, os_, oh = _weights(name, "weights_out", weights_out, seqs, heads)
-    desc = _EVICT.pack(wp, op, ws, wh, os_, oh, out_table.data_ptr(), out_table.stride(0), out_table.shape[1],
-                       min(weights.shape[2], weights_out.shape[2]), new_lens.data_ptr(), kept.data_ptr(), budget,
-                       recent)
-    _queue(dev, lambda st: check(lib().spinn_cuda_cache_evict(cache, table, desc, st), "spinn_cuda_cache_evict"))
+    (_binding or _ops()).cache_evict(k_cache, v_cache, page_table, lens, weights, weights_out, out_table, new_lens,
+                                     kept, budget, recent)
 
 
 class Model:

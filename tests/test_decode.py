@@ -1,11 +1,19 @@
 """Decoder-serving operators without a GPU: argument checks of the C entry points (which come
 before any CUDA call), of the Python calls, and the host arithmetic that the kernels share."""
 import ctypes
+import struct
 
 import numpy as np
 import pytest
 
 from spinn_b200 import lib, runtime
+
+CACHE = struct.Struct("<QQqqqiiiiii")             # SpinnCudaCache
+TABLE = struct.Struct("<QQqii")                   # SpinnCudaPageTable
+APPEND = struct.Struct("<QQqqqqQii")              # SpinnCudaAppend
+ATTENTION = struct.Struct("<QQqqqqQQqqqqiifi")    # SpinnCudaAttention
+EVICT = struct.Struct("<QQqqqqQqiiQQii")          # SpinnCudaEvict
+LINEAR = struct.Struct("<QQQQQqqqqiiiiii")        # SpinnCudaLinear
 
 BUF = ctypes.create_string_buffer(1 << 16)  # never dereferenced: every call here is refused
 P = (ctypes.addressof(BUF) + 255) & ~255
@@ -14,14 +22,14 @@ P = (ctypes.addressof(BUF) + 255) & ~255
 def cache(**kw):
     f = dict(k=P, v=P, ps=16 * 2 * 64, ts=2 * 64, hs=64, dtype=lib.BF16, pages=9, page=16, heads=2, dim=64)
     f.update(kw)
-    return runtime._CACHE.pack(f["k"], f["v"], f["ps"], f["ts"], f["hs"], f["dtype"], f["pages"], f["page"],
+    return CACHE.pack(f["k"], f["v"], f["ps"], f["ts"], f["hs"], f["dtype"], f["pages"], f["page"],
                                f["heads"], f["dim"], 0)
 
 
 def table(**kw):
     f = dict(pages=P, lens=P, stride=4, seqs=3, wide=4)
     f.update(kw)
-    return runtime._TABLE.pack(f["pages"], f["lens"], f["stride"], f["seqs"], f["wide"])
+    return TABLE.pack(f["pages"], f["lens"], f["stride"], f["seqs"], f["wide"])
 
 
 def refused(fn, *args, match):
@@ -40,13 +48,13 @@ BAD_TABLES = [(dict(pages=0), "null"), (dict(lens=0), "null"), (dict(seqs=0), "p
 def append(**kw):
     f = dict(k=P, v=P, starts=0, tokens=3, ks=128)
     f.update(kw)
-    return runtime._APPEND.pack(f["k"], f["v"], f["ks"], 64, 128, 64, f["starts"], f["tokens"], 0)
+    return APPEND.pack(f["k"], f["v"], f["ks"], 64, 128, 64, f["starts"], f["tokens"], 0)
 
 
 def attention(**kw):
     f = dict(q=P, y=P, win=0, wout=0, cap=0, q_heads=4, qs=256, wis=0, wos=0)
     f.update(kw)
-    return runtime._ATTENTION.pack(f["q"], f["y"], f["qs"], 64, 256, 64, f["win"], f["wout"], f["wis"], 0, f["wos"], 0,
+    return ATTENTION.pack(f["q"], f["y"], f["qs"], 64, 256, 64, f["win"], f["wout"], f["wis"], 0, f["wos"], 0,
                                    f["cap"], f["q_heads"], 0.125, 0)
 
 
@@ -54,7 +62,7 @@ def evict(**kw):
     f = dict(win=P, wout=P + 8192, out=P + 256, stride=4, wide=4, cap=64, new=P + 64, kept=P + 128, budget=16, recent=0,
              wis=128, wos=128)
     f.update(kw)
-    return runtime._EVICT.pack(f["win"], f["wout"], f["wis"], 64, f["wos"], 64, f["out"], f["stride"], f["wide"],
+    return EVICT.pack(f["win"], f["wout"], f["wis"], 64, f["wos"], 64, f["out"], f["stride"], f["wide"],
                                f["cap"], f["new"], f["kept"], f["budget"], f["recent"])
 
 
@@ -119,32 +127,55 @@ def test_python_calls_refuse_host_tensors():
     with pytest.raises(TypeError, match="CUDA"):
         runtime.paged_attention(q, k, k, t, n, q)
     with pytest.raises(TypeError, match="CUDA"):
-        runtime.cache_evict(k, k, t, n, w, w, t, n, n, 4)
+        runtime.cache_evict(k, k, t, n, w, w, t, n, torch.zeros(1, 2, 4, dtype=torch.int32), 4)
 
 
-def test_python_descriptors_check_shapes_and_types():
+def test_python_calls_check_shapes_and_types():
+    """Checked before the device, so that host tensors do."""
     torch = pytest.importorskip("torch")
-    runtime._torch_module()
     k = torch.zeros(4, 16, 2, 64)
-    with pytest.raises(ValueError, match="one shape"):
-        runtime._cache_desc("x", k, k[..., :32])
-    with pytest.raises(ValueError, match="one shape"):
-        runtime._cache_desc("x", k, torch.zeros(4, 2, 16, 64).transpose(1, 2))
-    with pytest.raises(TypeError, match="float64"):
-        runtime._cache_desc("x", k.double(), k.double())
-    with pytest.raises(ValueError, match="contiguous"):
-        runtime._cache_desc("x", k[..., ::2], k[..., ::2])
-    t = torch.zeros(3, 5, dtype=torch.int32)
-    with pytest.raises(TypeError, match="int32"):
-        runtime._table_desc("x", t.long(), t[:, 0])
-    with pytest.raises(ValueError, match="lens"):
-        runtime._table_desc("x", t, torch.zeros(2, dtype=torch.int32))
-    with pytest.raises(ValueError, match="contiguous"):
-        runtime._table_desc("x", t.t(), torch.zeros(5, dtype=torch.int32))
-    with pytest.raises(TypeError, match="float32"):
-        runtime._weights("x", "weights", torch.zeros(1, 2, 3, dtype=torch.float16), 1, 2)
-    with pytest.raises(TypeError, match="type"):
-        runtime._rows("x", "q", torch.zeros(1, 2, 64, dtype=torch.float16), k, (1, 2, 64))
+    t, n = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    q = torch.zeros(1, 2, 64)
+    w = torch.zeros(1, 2, 32)
+    kept = torch.zeros(1, 2, 4, dtype=torch.int32)
+
+    def attend(kc=k, vc=None, table=t, lens=n, x=q, y=q, win=None, wout=None, scale=None):
+        runtime.paged_attention(x, kc, kc if vc is None else vc, table, lens, y, scale, win, wout)
+
+    for bad, err, match in [
+            (dict(vc=k[..., :32]), ValueError, "one shape"),
+            (dict(vc=torch.zeros(4, 2, 16, 64).transpose(1, 2)), ValueError, "one shape"),
+            (dict(vc=k.half()), ValueError, "one shape"), (dict(kc=k.double()), TypeError, "float32"),
+            (dict(kc=k[..., ::2]), ValueError, "contiguous"), (dict(kc=k[0]), ValueError, "pages"),
+            (dict(table=t.long()), TypeError, "int32"), (dict(lens=n.long()), TypeError, "int32"),
+            (dict(table=torch.zeros(2, 2, dtype=torch.int32)), ValueError, "lens"),
+            (dict(table=torch.zeros(2, 4, dtype=torch.int32)[:1, ::2]), ValueError, "contiguous"),
+            (dict(x=q.half()), TypeError, "type"), (dict(y=q.half()), TypeError, "type"),
+            (dict(x=q[0]), ValueError, "q must"), (dict(x=torch.zeros(2, 2, 64)), ValueError, "q must"),
+            (dict(y=torch.zeros(1, 3, 64)), ValueError, "y must"), (dict(y=torch.zeros(1, 2, 128)[..., ::2]), ValueError, "y"),
+            (dict(win=w), ValueError, "without"), (dict(wout=w.half()), TypeError, "float32"),
+            (dict(wout=w[:, :1]), ValueError, "weights_out"), (dict(wout=w, win=w[0]), ValueError, "weights"),
+            (dict(scale="x"), TypeError, None)]:
+        with pytest.raises(err, match=match):
+            attend(**bad)
+    with pytest.raises(TypeError, match="torch tensor"):
+        attend(x=np.zeros((1, 2, 64), np.float32))
+    with pytest.raises(ValueError, match="without starts"):
+        runtime.cache_append(torch.zeros(2, 2, 64), torch.zeros(2, 2, 64), k, k, t, n)
+    with pytest.raises(ValueError, match="starts"):
+        runtime.cache_append(q, q, k, k, t, n, torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(TypeError, match="starts"):
+        runtime.cache_append(q, q, k, k, t, n, torch.zeros(2))
+    with pytest.raises(ValueError, match="v must"):
+        runtime.cache_append(q, torch.zeros(1, 2, 63), k, k, t, n)
+    for bad, err, match in [
+            (dict(kept=kept[..., :3]), ValueError, "kept"), (dict(new=n.long()), TypeError, "int32"),
+            (dict(new=torch.zeros(2, dtype=torch.int32)), ValueError, "new_lens"), (dict(out=t[0]), ValueError, "out_table"),
+            (dict(budget=2 ** 40), ValueError, "range"), (dict(budget="x"), TypeError, None)]:
+        f = dict(out=t, new=n.clone(), kept=kept, budget=4)
+        f.update(bad)
+        with pytest.raises(err, match=match):
+            runtime.cache_evict(k, k, t, n, w, w, f["out"], f["new"], f["kept"], f["budget"])
 
 
 # ------------------------------------------------------------------ shared host arithmetic
@@ -191,7 +222,7 @@ def test_attention_shares_cover_the_work_once():
 def linear(**kw):
     f = dict(x=P, w=P, b=0, r=0, y=P, ldx=64, ldw=64, ldr=0, ldy=32, m=4, n=32, k=64, dtype=lib.BF16, act=0)
     f.update(kw)
-    return runtime._LINEAR.pack(f["x"], f["w"], f["b"], f["r"], f["y"], f["ldx"], f["ldw"], f["ldr"], f["ldy"], f["m"],
+    return LINEAR.pack(f["x"], f["w"], f["b"], f["r"], f["y"], f["ldx"], f["ldw"], f["ldr"], f["ldy"], f["m"],
                                 f["n"], f["k"], f["dtype"], f["act"], 0)
 
 
@@ -219,6 +250,18 @@ def test_linear_workspace_holds_the_rows_that_are_off_alignment():
 
 def test_python_linear_refuses_what_does_not_match():
     torch = pytest.importorskip("torch")
-    x = torch.zeros(2, 8, dtype=torch.float16)
+    h = lambda *shape: torch.zeros(*shape, dtype=torch.float16)  # noqa: E731
     with pytest.raises(TypeError, match="CUDA"):
-        runtime.linear(x, x, torch.zeros(2, 2, dtype=torch.float16))
+        runtime.linear(h(2, 8), h(4, 8), h(2, 4))
+    for args, err, match in [((h(2, 8), h(4, 9), h(2, 4)), ValueError, r"\[m, k\]"),
+                             ((h(2, 8), h(4, 8), h(2, 5)), ValueError, r"\[m, k\]"), ((h(8), h(4, 8), h(2, 4)), ValueError, None),
+                             ((h(2, 8), h(4, 8).bfloat16(), h(2, 4)), TypeError, "float16"),
+                             ((h(2, 8).float(), h(4, 8).float(), h(2, 4).float()), TypeError, "float16"),
+                             ((h(2, 8), h(4, 8), h(2, 4), h(5)), ValueError, "bias"),
+                             ((h(2, 8), h(4, 8), h(2, 4), h(8)[::2]), ValueError, "bias"),
+                             ((h(2, 8), h(4, 8), h(2, 4), None, h(2, 5)), ValueError, "residual"),
+                             ((h(2, 16)[:, ::2], h(4, 8), h(2, 4)), ValueError, "contiguous"),
+                             ((h(2, 8), h(4, 8), h(4, 2).t()), ValueError, "contiguous"),
+                             ((h(2, 8), h(4, 8), h(2, 4), None, None, "tanh"), ValueError, "act")]:
+        with pytest.raises(err, match=match):
+            runtime.linear(*args)
