@@ -42,7 +42,8 @@ struct LinearParams {
   int m, n, k;
   int act;
   int num_kb, tiles_m, tiles_n, num_tiles;
-  bool vec;
+  bool vec;    // rows of x and w on 16-byte boundaries
+  bool vec_y;  // rows of y and the residual on 16-byte boundaries
   unsigned* err;
 };
 
@@ -61,23 +62,33 @@ __device__ __forceinline__ T round_to(float x) {
     return __float2bfloat16_rn(x);
 }
 
-// The activations of the fp32 accumulator.  SiLU and the tanh form share v / (1 + e^-z): the tanh
-// form is 0.5 v (1 + tanh u) = v / (1 + e^(-2 u)).  __expf's error (2 ulp plus 2^-22 |z|) is far
-// below the rounding of y.
-__device__ __forceinline__ float activate(float v, int act) {
+// The activations of the fp32 accumulators, chosen once per block of values: a switch per value
+// cost a third of a whole launch (4096 x 4096 x 8192 with SiLU: 234 us, 207 us without it).  SiLU
+// and the tanh form share v / (1 + e^-z): the tanh form is 0.5 v (1 + tanh u) = v / (1 + e^(-2 u)).
+// The fast exponential and quotient are off by a few ulp of fp32, far below the rounding of y.
+__device__ __forceinline__ float sigmoid_times(float v, float z) { return __fdividef(v, 1.0f + __expf(-z)); }
+template <int N>
+__device__ __forceinline__ void activate(float (&v)[N], int act) {
   switch (act) {
     case 1:
-      return v < 0.0f ? 0.0f : v;
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
+      break;
     case 3:
-      return v / (1.0f + __expf(-v));
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = sigmoid_times(v[i], v[i]);
+      break;
     case SPINN_CUDA_ACT_GELU:
-      return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-    case SPINN_CUDA_ACT_GELU_TANH: {
-      const float u = 1.5957691216057308f * (v + 0.044715f * v * v * v);  // 2 sqrt(2 / pi) (...)
-      return v / (1.0f + __expf(-u));
-    }
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = 0.5f * v[i] * (1.0f + erff(v[i] * 0.70710678118654752f));
+      break;
+    case SPINN_CUDA_ACT_GELU_TANH:
+#pragma unroll
+      for (int i = 0; i < N; ++i)  // 2 sqrt(2 / pi) (v + 0.044715 v^3)
+        v[i] = sigmoid_times(v[i], 1.5957691216057308f * (v[i] + 0.044715f * v[i] * v[i] * v[i]));
+      break;
     default:
-      return v;
+      break;
   }
 }
 
@@ -164,13 +175,13 @@ __global__ void __launch_bounds__(kRowWarps * 32) linear_rows_kernel(const Linea
   for (int i = threadIdx.x; i < NT * 8 * 16; i += kRowWarps * 32) {
     const int row = i >> 4, n = n0 + (i & 15);
     if (row >= p.m || n >= p.n) continue;
-    float v = 0.0f;
+    float v[1] = {0.0f};
 #pragma unroll
-    for (int s = 0; s < kRowWarps; ++s) v += part[s][row][i & 15];
-    if (p.bias) v += to_float(static_cast<const T*>(p.bias)[n]);
-    v = activate(v, p.act);
-    if (p.res) v += to_float(static_cast<const T*>(p.res)[row * p.ldr + n]);
-    static_cast<T*>(p.y)[row * p.ldy + n] = round_to<T>(v);
+    for (int s = 0; s < kRowWarps; ++s) v[0] += part[s][row][i & 15];
+    if (p.bias) v[0] += to_float(static_cast<const T*>(p.bias)[n]);
+    activate(v, p.act);
+    if (p.res) v[0] += to_float(static_cast<const T*>(p.res)[row * p.ldr + n]);
+    static_cast<T*>(p.y)[row * p.ldy + n] = round_to<T>(v[0]);
   }
 }
 
@@ -232,11 +243,14 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
 }
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t cluster_size() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
@@ -247,24 +261,51 @@ __device__ __forceinline__ bool warp_wait_bar(uint64_t* bar, uint32_t parity, vo
 }
 __device__ __forceinline__ bool warp_abort(volatile int* abort) { return __any_sync(0xffffffffu, *abort != 0); }
 
+// Barrier of the four epilogue warps of one group.
+__device__ __forceinline__ void group_sync(int group) {
+  asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory");
+}
+template <typename T>
+union Pack {
+  uint4 u;
+  T t[8];
+  __device__ Pack() {}
+};
+
+template <typename T>
+union Pair {
+  uint32_t u;
+  T t[2];
+  __device__ Pair() {}
+};
+
 constexpr int kTileThreads = 384;  // producer, MMA, TMEM and a spare warp, eight epilogue warps
 
 // BN: rows of x of a tile.  PAIR 2: a CTA pair works on 256 rows of w with one cta_group::2 MMA
 // stream, each CTA holding its 128 rows of w and half of the rows of x.  SPL: the CTAs of a
 // cluster share one tile and split its k.
+//
+// A stage holds 128 elements of k, two 128-byte swizzle spans: with one span per stage the
+// barrier handoffs showed (4096 x 4096 x 8192 without activation: 207 us, 178 us with two).
 template <int BN_, int PAIR_, bool SPL_>
 struct LinCfg {
   static constexpr int BN = BN_, PAIR = PAIR_;
   static constexpr bool SPL = SPL_;
-  static constexpr int BK = 64;                     // 128-byte rows: one swizzle span
-  static constexpr int A_STAGE = 128 * 128, B_STAGE = BN / PAIR * 128, STAGE = A_STAGE + B_STAGE;
-  static constexpr int FIT = (222 * 1024) / STAGE;
-  static constexpr int STAGES = FIT > 10 ? 10 : FIT;
+  static constexpr int BK = 128, SPAN = 64;  // elements of k per stage and per swizzle span
+  static constexpr int A_SPAN = 128 * 128, B_SPAN = BN / PAIR * 128;
+  static constexpr int A_STAGE = 2 * A_SPAN, B_STAGE = 2 * B_SPAN, STAGE = A_STAGE + B_STAGE;
+  static constexpr int PART = SPL ? BN * 128 * 4 : 0;  // partial sums received from the cluster
+  // The epilogue's staging, [16 rows of x][128 rows of w] per group of four warps: y leaves in
+  // 16-byte pieces of 256-byte row segments.
+  static constexpr int STG_PITCH = 128 + 4, STG = SPL ? 0 : 2 * 16 * STG_PITCH * 4;
+  static constexpr int FIT = (222 * 1024 - PART - STG) / STAGE;
+  static constexpr int STAGES = FIT > 6 ? 6 : FIT;
   static constexpr int NACC = SPL ? 1 : 2;          // accumulators: the epilogue drains one while the other fills
   static constexpr int COLS = NACC * BN < 32 ? 32 : NACC * BN;
-  static constexpr int SMEM = STAGES * STAGE + 512 + 1024;
+  static constexpr int SMEM = STAGES * STAGE + PART + STG + 512 + 1024;
   static_assert(COLS <= 512, "TMEM");
-  static_assert(!SPL || (PAIR == 1 && STAGES * STAGE >= BN * 128 * 4), "partial tiles reuse the stages");
+  static_assert(STAGES >= 2, "pipeline needs two stages");
+  static_assert(!SPL || PAIR == 1, "a cluster is either a pair or a split");
 };
 
 template <typename T, typename C>
@@ -277,7 +318,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = smem + STAGES * C::A_STAGE;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * C::STAGE);
+  float* part = reinterpret_cast<float*>(smem + STAGES * C::STAGE);  // [rank][slot][128 rows of w]
+  float* staging = reinterpret_cast<float*>(smem + STAGES * C::STAGE + C::PART);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * C::STAGE + C::PART + C::STG);
   uint64_t* empty = full + STAGES;
   uint64_t* tfull = empty + STAGES;
   uint64_t* tempty = tfull + NACC;
@@ -321,6 +364,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   tc_fence_before();
   __syncthreads();
   if constexpr (PAIR == 2) cluster_sync();  // the peer's barriers are initialised before use
+  if constexpr (SPL) cluster_arrive();      // waited for before the first store to another CTA
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   griddep_launch_dependents();
@@ -352,13 +396,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             armed |= 1u << s;
             armed_ph = (armed_ph & ~(1u << s)) | (ph << s);
           }
-          if constexpr (PAIR == 2) {
-            const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
-            tma_load_2d_pair(&mapW, bar, sA + s * C::A_STAGE, kb * C::BK, w_row);
-            tma_load_2d_pair(&mapX, bar, sB + s * C::B_STAGE, kb * C::BK, x_row);
-          } else {
-            tma_load_2d(&mapW, &full[s], sA + s * C::A_STAGE, kb * C::BK, w_row);
-            tma_load_2d(&mapX, &full[s], sB + s * C::B_STAGE, kb * C::BK, x_row);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // the second span may lie wholly past k: it reads as zeros
+            uint8_t *a = sA + s * C::A_STAGE + h * C::A_SPAN, *b = sB + s * C::B_STAGE + h * C::B_SPAN;
+            const int k = kb * C::BK + h * C::SPAN;
+            if constexpr (PAIR == 2) {
+              const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+              tma_load_2d_pair(&mapW, bar, a, k, w_row);
+              tma_load_2d_pair(&mapX, bar, b, k, x_row);
+            } else {
+              tma_load_2d(&mapW, &full[s], a, k, w_row);
+              tma_load_2d(&mapX, &full[s], b, k, x_row);
+            }
           }
         }
         __syncwarp();
@@ -399,10 +448,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
           for (int j = 0; j < C::BK / 16; ++j) {
             const uint32_t acc = kb != kb0 || j != 0 ? 1u : 0u;
+            const uint64_t aj = a + (j >> 2) * (C::A_SPAN >> 4) + 2 * (j & 3);
+            const uint64_t xj = x + (j >> 2) * (C::B_SPAN >> 4) + 2 * (j & 3);
             if constexpr (PAIR == 2)
-              umma_f16_pair(tmem + b * BN, a + 2 * j, x + 2 * j, idesc, acc);
+              umma_f16_pair(tmem + b * BN, aj, xj, idesc, acc);
             else
-              umma_f16(tmem + b * BN, a + 2 * j, x + 2 * j, idesc, acc);
+              umma_f16(tmem + b * BN, aj, xj, idesc, acc);
           }
           if constexpr (PAIR == 2) {
             umma_commit_pair(mapa_shared(smem_u32(&empty[s]), 0));
@@ -442,6 +493,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     // ---- epilogue: warp pairs share a TMEM lane quarter and alternate over its column chunks
     constexpr int CW = 16;  // columns (rows of x) per step
     const int quarter = warp & 3, half = (warp - 4) >> 2;
+    if constexpr (SPL) cluster_wait();  // the cluster's other CTAs run: their shared memory may be written
     int it = 0;
     for (int t = unit0; t < p.num_tiles; t += step, ++it) {
       int tm, tn;
@@ -455,29 +507,94 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       for (int c = half * CW; c < BN && m0 + c < p.m; c += 2 * CW) {
         uint32_t r[CW];
         tmem_ld_32x32b_x16(tmem + b * BN + c + ((uint32_t)(quarter * 32) << 16), r);
+        const int rows = min(CW, p.m - m0 - c);
         if constexpr (SPL) {
+          // rows of x in groups of four, group g finished by rank g % splits at slot g / splits
           tmem_ld_wait();
-          float* part = reinterpret_cast<float*>(smem) + c * 128 + quarter * 32 + lane;
+          const uint32_t mine = smem_u32(part) + (rank * (BN / 4 / splits) * 128 + quarter * 32 + lane) * 16;
 #pragma unroll
-          for (int i = 0; i < CW; ++i) part[i * 128] = __uint_as_float(r[i]);
+          for (int i = 0; i < CW; i += 4) {
+            const uint32_t g = (c + i) >> 2, to = g & (splits - 1), slot = g / splits;
+            if (i < rows) st_cluster_v4(mapa_shared(mine + slot * 2048, to), r[i], r[i + 1], r[i + 2], r[i + 3]);
+          }
         } else {
-          const int rows = min(CW, p.m - m0 - c);
-          T res[CW];
-          if (p.res && n < p.n) {
-            const T* src = static_cast<const T*>(p.res) + (long long)(m0 + c) * p.ldr + n;
+          // this thread's part of the output: eight consecutive n of two rows of x
+          const int on = (tn * PAIR + (PAIR == 2 ? rank : 0)) * 128 + (lane & 15) * 8;
+          const int orow = quarter * 4 + (lane >> 4);
+          uint4 res[2];
+          if (p.res && p.vec_y && on + 8 <= p.n) {
 #pragma unroll
-            for (int i = 0; i < CW; ++i)
-              if (i < rows) res[i] = src[i * p.ldr];
+            for (int j = 0; j < 2; ++j)
+              if (orow + 2 * j < rows)
+                res[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.res) +
+                                                              (long long)(m0 + c + orow + 2 * j) * p.ldr + on));
           }
           tmem_ld_wait();
-          if (n < p.n) {
-            T* dst = static_cast<T*>(p.y) + (long long)(m0 + c) * p.ldy + n;
+          float v[CW];
 #pragma unroll
-            for (int i = 0; i < CW; ++i) {
-              if (i >= rows) break;
-              float v = activate(__uint_as_float(r[i]) + bias, p.act);
-              if (p.res) v += to_float(res[i]);
-              dst[i * p.ldy] = round_to<T>(v);
+          for (int i = 0; i < CW; ++i) v[i] = __uint_as_float(r[i]) + bias;
+          activate(v, p.act);
+          float* stage = staging + half * 16 * C::STG_PITCH;
+          group_sync(half);  // the previous step's values have been read
+#pragma unroll
+          for (int i = 0; i < CW; ++i) stage[i * C::STG_PITCH + quarter * 32 + lane] = v[i];
+          group_sync(half);
+          if (p.vec_y) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int row = orow + 2 * j;
+              if (row >= rows || on >= p.n) continue;
+              const float4* src = reinterpret_cast<const float4*>(stage + row * C::STG_PITCH + (lane & 15) * 8);
+              const float4 lo = src[0], hi = src[1];
+              float o[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+              T* dst = static_cast<T*>(p.y) + (long long)(m0 + c + row) * p.ldy + on;
+              if (on + 8 <= p.n) {
+                Pack<T> x;
+                if (p.res) {
+                  x.u = res[j];
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) o[i] += to_float(x.t[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x.t[i] = round_to<T>(o[i]);
+                *reinterpret_cast<uint4*>(dst) = x.u;
+              } else {
+                const T* extra = static_cast<const T*>(p.res) + (p.res ? (long long)(m0 + c + row) * p.ldr + on : 0);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                  if (on + i < p.n) dst[i] = round_to<T>(p.res ? o[i] + to_float(extra[i]) : o[i]);
+              }
+            }
+          } else {
+            // rows off alignment: 4-byte words at the row's own parity, its ends in single elements
+            const int n0 = (tn * PAIR + (PAIR == 2 ? rank : 0)) * 128, width = min(128, p.n - n0);
+            for (int q = 0; q < 4; ++q) {
+              const int row = quarter * 4 + q;
+              if (row >= rows) break;
+              T* dst = static_cast<T*>(p.y) + (long long)(m0 + c + row) * p.ldy + n0;
+              const T* extra = p.res ? static_cast<const T*>(p.res) + (long long)(m0 + c + row) * p.ldr + n0 : nullptr;
+              const float* src = stage + row * C::STG_PITCH;
+              const int odd = ((uintptr_t)dst >> 1) & 1;
+#pragma unroll
+              for (int j = 0; j < 3; ++j) {
+                const int e = 2 * (lane + 32 * j) - odd;
+                if (e >= width || (j == 2 && e > 127)) continue;
+                const bool first = e >= 0, second = e + 1 < width;
+                float o0 = first ? src[e] : 0.0f, o1 = second ? src[e + 1] : 0.0f;
+                if (extra) {
+                  if (first) o0 += to_float(extra[e]);
+                  if (second) o1 += to_float(extra[e + 1]);
+                }
+                Pair<T> x;
+                x.t[0] = round_to<T>(o0);
+                x.t[1] = round_to<T>(o1);
+                if (first && second)
+                  *reinterpret_cast<uint32_t*>(dst + e) = x.u;
+                else if (first)
+                  dst[e] = x.t[0];
+                else
+                  dst[e + 1] = x.t[1];
+              }
             }
           }
         }
@@ -494,26 +611,45 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
 
   if constexpr (SPL) {
-    // Partial tiles, [row of x][128 rows of w] in every CTA's shared memory, added in rank order;
-    // each CTA finishes its share of the rows of x.
-    __syncthreads();
-    cluster_sync();
+    // Every CTA has sent its partial sums to the CTAs that finish them, which add them in rank
+    // order out of their own shared memory.
+    if (warp < 4) cluster_wait();
+    cluster_arrive();
+    cluster_wait();
     int tm, tn;
     decode(unit0, &tm, &tn);
-    const int rows = min(BN, p.m - tm * BN);
-    const int c0 = rows * (int)rank / (int)splits, c1 = rows * ((int)rank + 1) / (int)splits;
-    const uint32_t base = smem_u32(smem);
-    for (int i = c0 * 128 + threadIdx.x; i < c1 * 128; i += kTileThreads) {
-      const int n = tn * 128 + (i & 127), m = tm * BN + (i >> 7);
+    const int rows = min(BN, p.m - tm * BN), groups = (rows + 3) >> 2;
+    const int mine = (groups - (int)rank + (int)splits - 1) / (int)splits;  // groups rank, rank + splits, ...
+    const float4* sums = reinterpret_cast<const float4*>(part);
+    const int plane = BN / 4 / (int)splits * 128;
+    for (int i = threadIdx.x; i < mine * 128; i += kTileThreads) {
+      const int n = tn * 128 + (i & 127), row = ((i >> 7) * (int)splits + (int)rank) * 4, m = tm * BN + row;
       if (n >= p.n) continue;
-      float v = 0.0f;
-      for (uint32_t j = 0; j < splits; ++j) v += ld_cluster_f32(mapa_shared(base + i * 4, j));
-      if (p.bias) v += to_float(static_cast<const T*>(p.bias)[n]);
-      v = activate(v, p.act);
-      if (p.res) v += to_float(static_cast<const T*>(p.res)[m * p.ldr + n]);
-      static_cast<T*>(p.y)[m * p.ldy + n] = round_to<T>(v);
+      float res[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (p.res) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (row + e < rows) res[e] = to_float(static_cast<const T*>(p.res)[(m + e) * p.ldr + n]);
+      }
+      const float bias = p.bias ? to_float(static_cast<const T*>(p.bias)[n]) : 0.0f;
+      float4 x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = j < (int)splits ? sums[j * plane + i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[0] += x[j].x;
+        v[1] += x[j].y;
+        v[2] += x[j].z;
+        v[3] += x[j].w;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += bias;
+      activate(v, p.act);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (row + e < rows) static_cast<T*>(p.y)[(m + e) * p.ldy + n] = round_to<T>(p.res ? v[e] + res[e] : v[e]);
     }
-    cluster_sync();  // the others have read this CTA's part
   }
   __syncthreads();
   if constexpr (PAIR == 2) cluster_sync();  // no CTA leaves while its peer may use its memory
@@ -544,7 +680,7 @@ LinearPlan linear_plan(const LinearParams& p, int sms) {
   pl.copy_w = !tma_rows(p.w, p.ldw);
   pl.x_bytes = pl.copy_x ? (pitch * p.m + 255) / 256 * 256 : 0;
   pl.w_bytes = pl.copy_w ? (pitch * p.n + 255) / 256 * 256 : 0;
-  const int kb = (p.k + 63) / 64, tn = (p.n + 127) / 128;
+  const int kb = (p.k + 127) / 128, tn = (p.n + 127) / 128;
   auto tiles = [&](int bn) { return (long long)((p.m + bn - 1) / bn) * tn; };
   // CTA pairs of 256 x 256 where they fill the GPU; else the widest tile that fills it; else the
   // narrowest one that holds the rows, with k split over a cluster
@@ -555,7 +691,7 @@ LinearPlan linear_plan(const LinearParams& p, int sms) {
     return pl;
   }
   pl.bn = p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
-  while (pl.split < 8 && tiles(pl.bn) * pl.split * 2 <= sms && kb >= pl.split * 2 * 4) pl.split *= 2;
+  while (pl.split < 8 && tiles(pl.bn) * pl.split * 2 <= sms && kb >= pl.split * 2 * 2) pl.split *= 2;
   return pl;
 }
 
@@ -563,7 +699,7 @@ template <typename T, typename C>
 int launch_tiles(const LinearParams& p0, const LinearPlan& pl, const void* x, long long ldx, const void* w, long long ldw,
                  int sms, cudaStream_t st) {
   LinearParams p = p0;
-  p.num_kb = (p.k + 63) / 64;
+  p.num_kb = (p.k + C::BK - 1) / C::BK;
   p.tiles_m = (p.m + C::BN - 1) / C::BN;
   p.tiles_n = (p.n + 128 * C::PAIR - 1) / (128 * C::PAIR);
   const long long tiles = (long long)p.tiles_m * p.tiles_n;
@@ -571,9 +707,9 @@ int launch_tiles(const LinearParams& p0, const LinearPlan& pl, const void* x, lo
   p.num_tiles = (int)tiles;
   CUtensorMap mw, mx;
   const bool half = std::is_same<T, __half>::value;
-  int rc = encode_tiled_2d_16(&mw, w, p.k, p.n, (uint64_t)ldw * 2, C::BK, 128, half);
+  int rc = encode_tiled_2d_16(&mw, w, p.k, p.n, (uint64_t)ldw * 2, C::SPAN, 128, half);
   if (rc) return rc;
-  rc = encode_tiled_2d_16(&mx, x, p.k, p.m, (uint64_t)ldx * 2, C::BK, C::BN / C::PAIR, half);
+  rc = encode_tiled_2d_16(&mx, x, p.k, p.m, (uint64_t)ldx * 2, C::SPAN, C::BN / C::PAIR, half);
   if (rc) return rc;
   auto* kernel = linear_tile_kernel<T, C>;
   SPINN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
@@ -674,6 +810,7 @@ int linear_params(const SpinnCudaLinear* l, LinearParams* p) {
   p->k = l->k;
   p->act = l->act;
   p->vec = tma_rows(l->x, l->x_stride) && tma_rows(l->w, l->w_stride);
+  p->vec_y = tma_rows(l->y, l->y_stride) && (!l->residual || tma_rows(l->residual, l->residual_stride));
   p->err = nullptr;
   return 0;
 }
