@@ -194,19 +194,54 @@ struct PitchParams {
   int rows[2];
   int k, pitch;
 };
+// A thread makes 16-byte pieces out of the two aligned 16-byte words that hold them: a word is
+// read only when it holds an element of the row, so nothing outside the rows' own words is touched.
 __global__ void __launch_bounds__(256) pitch_kernel(const PitchParams p) {
   griddep_launch_dependents();
   griddep_wait();
   const int o = blockIdx.y;
-  for (int r = blockIdx.x; r < p.rows[o]; r += gridDim.x) {
-    const uint16_t* s = p.src[o] + r * p.ld[o];
-    uint16_t* d = p.dst[o] + (long long)r * p.pitch;
-    for (int c = threadIdx.x * 8; c < p.pitch; c += 256 * 8) {
-      uint32_t h[8];
+  const int pieces = p.pitch >> 3;
+  const long long total = (long long)p.rows[o] * pieces;
+  constexpr int U = 4;
+  for (long long i0 = (long long)blockIdx.x * 256 * U + threadIdx.x; i0 < total; i0 += (long long)gridDim.x * 256 * U) {
+    uint4 lo[U], hi[U];
+    int shift[U], valid[U];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = c + i < p.k ? s[c + i] : 0;
-      *reinterpret_cast<uint4*>(d + c) =
-          make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+    for (int u = 0; u < U; ++u) {
+      const long long i = i0 + u * 256;
+      lo[u] = hi[u] = make_uint4(0, 0, 0, 0);
+      valid[u] = shift[u] = 0;
+      if (i < total) {
+        const int r = (int)(i / pieces), c = (int)(i - (long long)r * pieces) * 8;
+        const uintptr_t at = reinterpret_cast<uintptr_t>(p.src[o] + r * p.ld[o] + c);
+        const uint4* word = reinterpret_cast<const uint4*>(at & ~uintptr_t(15));
+        shift[u] = (int)(at & 15) >> 1;  // elements
+        valid[u] = min(8, p.k - c);
+        lo[u] = __ldg(word);
+        if (shift[u] + valid[u] > 8) hi[u] = __ldg(word + 1);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long i = i0 + u * 256;
+      if (i >= total) continue;
+      // the 16 bytes at `shift` elements of lo : hi
+      uint32_t w[8] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w, hi[u].x, hi[u].y, hi[u].z, hi[u].w}, d[4];
+      const int whole = shift[u] >> 1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t a = 0, b = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (q == whole) {
+            a = w[j + q];
+            b = j + q + 1 < 8 ? w[j + q + 1] : 0;
+          }
+        d[j] = shift[u] & 1 ? __funnelshift_r(a, b, 16) : a;
+        const int left = valid[u] - 2 * j;  // elements of the row in this word
+        d[j] = left >= 2 ? d[j] : left == 1 ? d[j] & 0xffffu : 0u;
+      }
+      reinterpret_cast<uint4*>(p.dst[o])[i] = make_uint4(d[0], d[1], d[2], d[3]);
     }
   }
 }
@@ -611,44 +646,70 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
 
   if constexpr (SPL) {
-    // Every CTA has sent its partial sums to the CTAs that finish them, which add them in rank
-    // order out of their own shared memory.
-    if (warp < 4) cluster_wait();
-    cluster_arrive();
-    cluster_wait();
+    // Every CTA sends its partial sums to the CTAs that finish them, which add them in rank order
+    // out of their own shared memory.  A thread finishes two n of every sixth group of four rows;
+    // what it needs from global memory is asked for before the barrier.
     int tm, tn;
     decode(unit0, &tm, &tn);
     const int rows = min(BN, p.m - tm * BN), groups = (rows + 3) >> 2;
     const int mine = (groups - (int)rank + (int)splits - 1) / (int)splits;  // groups rank, rank + splits, ...
+    const int n = tn * 128 + 2 * (threadIdx.x & 63);
+    const bool one = n < p.n, two = n + 1 < p.n;
+    const float bias0 = p.bias && one ? to_float(static_cast<const T*>(p.bias)[n]) : 0.0f;
+    const float bias1 = p.bias && two ? to_float(static_cast<const T*>(p.bias)[n + 1]) : 0.0f;
+    const bool words = ((uintptr_t)p.y & 3) == 0 && (p.ldy & 1) == 0;
     const float4* sums = reinterpret_cast<const float4*>(part);
     const int plane = BN / 4 / (int)splits * 128;
-    for (int i = threadIdx.x; i < mine * 128; i += kTileThreads) {
-      const int n = tn * 128 + (i & 127), row = ((i >> 7) * (int)splits + (int)rank) * 4, m = tm * BN + row;
-      if (n >= p.n) continue;
-      float res[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (p.res) {
+    bool joined = false;
+    for (int g = threadIdx.x >> 6; g < mine || !joined; g += kTileThreads / 64) {
+      const int row = (g * (int)splits + (int)rank) * 4, m = tm * BN + row;
+      float res[4][2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (row + e < rows) res[e] = to_float(static_cast<const T*>(p.res)[(m + e) * p.ldr + n]);
+      for (int e = 0; e < 4; ++e) {
+        const bool live = p.res && g < mine && row + e < rows;
+        const T* src = static_cast<const T*>(p.res) + (live ? (long long)(m + e) * p.ldr + n : 0);
+        res[e][0] = live && one ? to_float(src[0]) : 0.0f;
+        res[e][1] = live && two ? to_float(src[1]) : 0.0f;
       }
-      const float bias = p.bias ? to_float(static_cast<const T*>(p.bias)[n]) : 0.0f;
-      float4 x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = j < (int)splits ? sums[j * plane + i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (!joined) {
+        if (warp < 4) cluster_wait();
+        cluster_arrive();
+        cluster_wait();
+        joined = true;
+      }
+      if (g >= mine || !one) continue;
+      float v[8] = {};
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[0] += x[j].x;
-        v[1] += x[j].y;
-        v[2] += x[j].z;
-        v[3] += x[j].w;
+        if (j >= (int)splits) break;
+        const float4 a = sums[j * plane + g * 128 + 2 * (threadIdx.x & 63)];
+        const float4 b = sums[j * plane + g * 128 + 2 * (threadIdx.x & 63) + 1];
+        v[0] += a.x;
+        v[1] += b.x;
+        v[2] += a.y;
+        v[3] += b.y;
+        v[4] += a.z;
+        v[5] += b.z;
+        v[6] += a.w;
+        v[7] += b.w;
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += bias;
+      for (int e = 0; e < 8; ++e) v[e] += e & 1 ? bias1 : bias0;
       activate(v, p.act);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (row + e < rows) static_cast<T*>(p.y)[(m + e) * p.ldy + n] = round_to<T>(p.res ? v[e] + res[e] : v[e]);
+      for (int e = 0; e < 4; ++e) {
+        if (row + e >= rows) continue;
+        T* dst = static_cast<T*>(p.y) + (long long)(m + e) * p.ldy + n;
+        Pair<T> x;
+        x.t[0] = round_to<T>(p.res ? v[2 * e] + res[e][0] : v[2 * e]);
+        x.t[1] = round_to<T>(p.res ? v[2 * e + 1] + res[e][1] : v[2 * e + 1]);
+        if (words && two) {
+          *reinterpret_cast<uint32_t*>(dst) = x.u;
+        } else {
+          dst[0] = x.t[0];
+          if (two) dst[1] = x.t[1];
+        }
+      }
     }
   }
   __syncthreads();
@@ -680,18 +741,33 @@ LinearPlan linear_plan(const LinearParams& p, int sms) {
   pl.copy_w = !tma_rows(p.w, p.ldw);
   pl.x_bytes = pl.copy_x ? (pitch * p.m + 255) / 256 * 256 : 0;
   pl.w_bytes = pl.copy_w ? (pitch * p.n + 255) / 256 * 256 : 0;
-  const int kb = (p.k + 127) / 128, tn = (p.n + 127) / 128;
-  auto tiles = [&](int bn) { return (long long)((p.m + bn - 1) / bn) * tn; };
-  // CTA pairs of 256 x 256 where they fill the GPU; else the widest tile that fills it; else the
-  // narrowest one that holds the rows, with k split over a cluster
-  const long long pair_tiles = (long long)((p.m + 255) / 256) * ((p.n + 255) / 256);
-  if (pair_tiles * 2 >= sms) {
-    pl.bn = 256;
-    pl.pair = 2;
-    return pl;
-  }
-  pl.bn = p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
-  while (pl.split < 8 && tiles(pl.bn) * pl.split * 2 <= sms && kb >= pl.split * 2 * 2) pl.split *= 2;
+  // Shape by estimated clocks, fitted to a sweep of every shape over 30 sizes (device time in a
+  // captured queue).  A stage of 128 k takes as long as its operands need to pass through shared
+  // memory twice (written by TMA, read by the MMA at 128 bytes a clock): about 870 clocks for a
+  // single CTA whatever its width up to 128, 950 and 1,150 for the pairs.  Around the stages lie
+  // the launch and first loads (2,600; 900 more for a cluster), and the last tile's epilogue.
+  // Splitting k pays when there are few tiles: it adds the exchange of the partial sums.
+  const int kb = (p.k + 127) / 128;
+  double best = 0;
+  auto consider = [&](int bn, int pair, int split) {
+    const long long tiles = (long long)((p.m + bn - 1) / bn) * ((p.n + 128 * pair - 1) / (128 * pair));
+    const long long waves = (tiles * pair * split + sms - 1) / sms;
+    if (split > 1 && (waves > 1 || kb < 2 * split)) return;
+    const double stage = pair == 1 ? 870.0 : bn == 256 ? 1150.0 : 950.0;
+    double clocks = 2600.0 + (pair * split > 1 ? 900.0 : 0.0) + (double)waves * ((kb + split - 1) / split) * stage;
+    clocks += bn * 30.0 + 300.0;
+    if (split > 1) clocks += 1100.0 + bn * 26.0 / split;
+    if (pl.bn == 0 || clocks < best) {
+      pl.bn = bn;
+      pl.pair = pair;
+      pl.split = split;
+      best = clocks;
+    }
+  };
+  for (int split = 1; split <= 8; split *= 2)
+    for (int bn = 32; bn <= 128; bn *= 2) consider(bn, 1, split);
+  consider(128, 2, 1);
+  consider(256, 2, 1);
   return pl;
 }
 
@@ -766,10 +842,12 @@ int linear_launch(const LinearParams& p, const LinearPlan& pl, void* ws, int sms
       w = c.dst[1];
       ldw = c.pitch;
     }
-    const int rc = launch_dependent(pitch_kernel, dim3(std::min(std::max(c.rows[0], c.rows[1]), sms * 8), 2), 256, 0, st, c);
+    const int rc = launch_dependent(pitch_kernel, dim3((unsigned)std::min<long long>(((long long)std::max(c.rows[0], c.rows[1]) * (c.pitch / 8) + 1023) / 1024, sms * 8), 2), 256, 0, st, c);
     if (rc) return rc;
   }
-  if (pl.pair == 2) return launch_tiles<T, LinCfg<256, 2, false>>(p, pl, x, ldx, w, ldw, sms, st);
+  if (pl.pair == 2)
+    return pl.bn == 256 ? launch_tiles<T, LinCfg<256, 2, false>>(p, pl, x, ldx, w, ldw, sms, st)
+                        : launch_tiles<T, LinCfg<128, 2, false>>(p, pl, x, ldx, w, ldw, sms, st);
   const bool spl = pl.split > 1;
 #define LINEAR_BN(W)                                                                        \
   if (pl.bn == W)                                                                           \
