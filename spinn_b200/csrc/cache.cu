@@ -167,6 +167,16 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
 }
 
 // ------------------------------------------------------------------ eviction
+__device__ __forceinline__ uint32_t cluster_nctas() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
 struct EvictParams {
   CacheView c;
   const float* win;
@@ -332,6 +342,216 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
   for (int j = n + tid; j < len; j += kSelThreads) wout[j] = 0.0f;
 }
 
+// The same choice where the weights of a (sequence, head) fit into the shared memory of a cluster,
+// which is nearly always: they are read once, and being copies, in place needs no staging.  The
+// digit counts are summed over the cluster through distributed shared memory, and the passes end
+// as soon as all of the threshold digit's keys are kept (with distinct weights mostly after
+// three).  Digits of 12 bits need one pass less, but their 4096 counts cost more to sum over the
+// cluster than a pass (20,000 clocks against 2,000).
+//
+// Bound by instructions, about two clocks per token on an SM, and by its chain of barriers: 16 x 8
+// heads of up to 4096 tokens take 9.7 us, 3 x 8 of up to 131072 33 us, where one CTA per head that
+// re-reads the weights takes 12.4 and 147.
+constexpr int kClThreads = 512, kClWarps = kClThreads / 32;
+constexpr int kClTokens = 26 * 1024;  // of one CTA: 208 KB of keys and weights
+
+__global__ void __launch_bounds__(kClThreads) evict_select_cluster_kernel(const EvictParams p) {
+  griddep_launch_dependents();
+  // this CTA's keys and then its weights, warp by warp: both, because a key does not give back a
+  // NaN's weight, and making keys out of weights in every pass took half of its time
+  extern __shared__ unsigned cached[];
+  __shared__ unsigned hist[4][256];
+  __shared__ unsigned mine[2][256];  // this CTA's digit counts, by parity of the pass
+  __shared__ int scan[8], warp_gt[kClWarps], warp_eq[kClWarps], total[2];
+  __shared__ unsigned sh_prefix;
+  __shared__ int sh_need, sh_count;
+  const int ctas = (int)cluster_nctas(), rank = ctas > 1 ? (int)cluster_ctarank() : 0;
+  const int pair = blockIdx.x / ctas;
+  const int s = pair / p.c.kv_heads, h = pair - s * p.c.kv_heads;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int all = ctas * kClThreads, me = rank * kClThreads + tid;
+  const int len = evict_length(p, s);
+  int* kept = p.kept + (long long)pair * p.budget;
+  const float* win = p.win + s * p.win_seq + h * p.win_head;
+  float* wout = p.wout + s * p.wout_seq + h * p.wout_head;
+  const int n = len < 0 ? 0 : min(len, p.budget);
+  if (me == 0 && h == 0) p.new_lens[s] = n;
+  for (int j = n + me; j < p.budget; j += all) kept[j] = -1;
+  if (len <= 0) return;
+  if (n == len) {  // everything stays
+    for (int j = me; j < n; j += all) {
+      kept[j] = j;
+      if (!p.same_weights) wout[j] = win[j];
+    }
+    return;
+  }
+  // Kept are the n largest keys, where a recent token's key is above every weight's and that of a
+  // slot past the end below.
+  const int old = len - min(p.recent, n);
+  // contiguous part of each warp, `steps` times 32 tokens
+  const int steps = (len + all - 1) / all;
+  const int i0 = (rank * kClWarps + warp) * steps * 32;
+  unsigned* keys = cached + warp * steps * 32 + lane;
+  unsigned* w = keys + kClThreads * steps;
+  // all of the weights are asked for at once
+  for (int j = 0; j < steps; ++j) {
+    const int i = i0 + j * 32 + lane;
+    if (i < len) cp_async_4(w + j * 32, win + i);
+  }
+  cp_async_wait_all();
+#pragma unroll 4
+  for (int j = 0; j < steps; ++j) {
+    const int i = i0 + j * 32 + lane;
+    keys[j * 32] = i < old ? weight_key(__uint_as_float(w[j * 32])) : i < len ? 0xffffffffu : 0u;
+  }
+  // threshold: of the keys whose bits under `mask` equal `prefix`, the first `ties` are kept, and
+  // all larger ones
+  unsigned prefix = 0, mask = 0;
+  int ties = n;
+  for (int shift = 24, pass = 0; shift >= 0; shift -= 8, ++pass) {
+    for (int q = tid; q < 4 * 256; q += kClThreads) hist[0][q] = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int j = 0; j < steps; ++j) {
+      const unsigned key = keys[j * 32];
+      if ((key & mask) == prefix) atomicAdd(&hist[warp & 3][(key >> shift) & 255], 1u);
+    }
+    __syncthreads();
+    if (tid < 256) mine[pass & 1][tid] = hist[0][tid] + hist[1][tid] + hist[2][tid] + hist[3][tid];
+    if (ctas > 1)
+      cluster_sync();
+    else
+      __syncthreads();
+    // thread t < 256 has digit 255 - t: an inclusive scan counts the keys from the largest on
+    unsigned count = 0, incl = 0;
+    if (tid < 256) {
+      if (ctas > 1) {
+        const uint32_t at = smem_u32(&mine[pass & 1][255 - tid]);
+        unsigned c[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) c[k] = k < ctas ? ld_cluster_u32(mapa_shared(at, k)) : 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) count += c[k];
+      } else {
+        count = mine[pass & 1][255 - tid];
+      }
+      incl = count;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const unsigned o = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += o;
+      }
+      if (lane == 31) scan[warp] = (int)incl;
+    }
+    __syncthreads();
+    if (tid < 256) {
+      incl += __reduce_add_sync(0xffffffffu, lane < warp ? scan[lane & 7] : 0);
+      if ((int)(incl - count) < ties && (int)incl >= ties) {
+        sh_prefix = prefix | (unsigned)(255 - tid) << shift;
+        sh_need = ties - (int)(incl - count);
+        sh_count = (int)count;
+      }
+    }
+    __syncthreads();
+    prefix = sh_prefix;
+    ties = sh_need;
+    mask |= 255u << shift;
+    if (sh_count == ties) break;
+  }
+  // keys above the threshold and at it, per warp
+  int gt = 0, eq = 0;
+#pragma unroll 4
+  for (int j = 0; j < steps; ++j) {
+    const unsigned key = keys[j * 32] & mask;
+    gt += key > prefix;
+    eq += key == prefix;
+  }
+  gt = __reduce_add_sync(0xffffffffu, gt);
+  eq = __reduce_add_sync(0xffffffffu, eq);
+  if (lane == 0) {
+    warp_gt[warp] = gt;
+    warp_eq[warp] = eq;
+  }
+  __syncthreads();
+  // larger keys and threshold keys before this warp's part
+  const int g = warp_gt[lane & (kClWarps - 1)], e = warp_eq[lane & (kClWarps - 1)];
+  int at = __reduce_add_sync(0xffffffffu, lane < warp ? g : 0);
+  int seen = __reduce_add_sync(0xffffffffu, lane < warp ? e : 0);
+  if (ctas > 1) {
+    if (warp == 0) {
+      const int a = __reduce_add_sync(0xffffffffu, lane < kClWarps ? g : 0);
+      const int b = __reduce_add_sync(0xffffffffu, lane < kClWarps ? e : 0);
+      if (lane == 0) {
+        total[0] = a;
+        total[1] = b;
+      }
+    }
+    cluster_sync();
+    int a = 0, b = 0;
+    if (lane < rank) {
+      a = (int)ld_cluster_u32(mapa_shared(smem_u32(&total[0]), lane));
+      b = (int)ld_cluster_u32(mapa_shared(smem_u32(&total[1]), lane));
+    }
+    at += __reduce_add_sync(0xffffffffu, a);
+    seen += __reduce_add_sync(0xffffffffu, b);
+    cluster_arrive();  // waited for before leaving: the totals have been read
+  }
+  at += min(seen, ties);
+  // Slots, 32 steps at a time: lane j holds the masks of step j, so that the steps' positions come
+  // from one scan instead of a chain over the steps.
+  const unsigned below = (1u << lane) - 1;
+  for (int j0 = 0; j0 < steps; j0 += 32) {
+    const int count = min(32, steps - j0);
+    unsigned more = 0, same = 0;
+#pragma unroll 4
+    for (int j = 0; j < count; ++j) {
+      const unsigned key = keys[(j0 + j) * 32] & mask;
+      const unsigned m = __ballot_sync(0xffffffffu, key > prefix), t = __ballot_sync(0xffffffffu, key == prefix);
+      if (lane == j) {
+        more = m;
+        same = t;
+      }
+    }
+    int before = __popc(same);
+    const int mine_eq = before;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, before, d);
+      if (lane >= d) before += o;
+    }
+    const int eqs = __shfl_sync(0xffffffffu, before, 31);
+    // the first `ties` threshold keys in all are kept
+    int take = min(mine_eq, max(0, ties - (seen + before - mine_eq)));
+    unsigned keep = more;
+    for (; take > 0; --take) {
+      keep |= same & (0u - same);
+      same &= same - 1;
+    }
+    int base = __popc(keep);
+    const int own = base;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, base, d);
+      if (lane >= d) base += o;
+    }
+    const int ks = __shfl_sync(0xffffffffu, base, 31);
+    base += at - own;
+#pragma unroll 4
+    for (int j = 0; j < count; ++j) {
+      const unsigned k = __shfl_sync(0xffffffffu, keep, j);
+      const int to = __shfl_sync(0xffffffffu, base, j) + __popc(k & below);
+      if (k >> lane & 1) {
+        kept[to] = i0 + (j0 + j) * 32 + lane;
+        wout[to] = __uint_as_float(w[(j0 + j) * 32]);
+      }
+    }
+    at += ks;
+    seen += eqs;
+  }
+  for (int j = n + me; j < len; j += all) wout[j] = 0.0f;
+  if (ctas > 1) cluster_wait();
+}
+
 // Offsets of a kept row's source and destination; false (error raised) when a page is bad.
 __device__ __forceinline__ bool evict_offsets(const EvictParams& p, int s, int h, int j, int from, long long* src,
                                               long long* dst) {
@@ -445,6 +665,65 @@ __global__ void __launch_bounds__(256) evict_shift_kernel(const EvictParams p, i
       if (to[q] >= 0) pool[to[q]] = r[q];
     __syncthreads();
   }
+}
+
+// Clusters of 1 .. 8 CTAs of the selection kernel, at their largest, that the device holds at once
+// (its GPCs do not divide evenly: 15 of eight, 22 of six, 26 of five on 148 SMs).
+int select_clusters(int device, int ctas) {
+  static std::mutex mu;
+  static std::map<std::pair<int, int>, int> known;
+  std::lock_guard<std::mutex> lk(mu);
+  int& n = known[{device, ctas}];
+  if (!n) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kClThreads);
+    cfg.dynamicSmemBytes = kClTokens * 8;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = ctas;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, evict_select_cluster_kernel, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = 1;
+    }
+  }
+  return n;
+}
+
+// As many CTAs per (sequence, head), up to a cluster of eight, as leave each 2048 tokens while all
+// clusters run at once; past the 212,992 tokens that eight hold, the kernel that re-reads the
+// weights.
+int launch_select(const EvictParams& p, int pairs, int device, cudaStream_t st) {
+  const int cap = std::min(cache_capacity(p.c.max_pages, p.c.page_size), p.wcap);
+  auto tokens = [&](int c) { return ((long long)cap + c * kClThreads - 1) / (c * kClThreads) * kClThreads; };
+  SPINN_CUDA_TRY(cudaFuncSetAttribute(evict_select_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      kClTokens * 8));
+  int ctas = std::max(1, std::min(8, cap / 2048));
+  while (ctas > 1 && pairs > select_clusters(device, ctas)) --ctas;
+  while (ctas < 8 && tokens(ctas) > kClTokens) ++ctas;
+  if (tokens(ctas) > kClTokens) {
+    evict_select_kernel<<<(unsigned)pairs, kSelThreads, 0, st>>>(p);
+    SPINN_CUDA_TRY(cudaGetLastError());
+    return 0;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(pairs * ctas));
+  cfg.blockDim = dim3(kClThreads);
+  cfg.dynamicSmemBytes = (size_t)tokens(ctas) * 8;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  SPINN_CUDA_TRY(cudaLaunchKernelEx(&cfg, evict_select_cluster_kernel, p));
+  return 0;
 }
 
 bool overlap(const void* a, size_t na, const void* b, size_t nb) {
@@ -578,8 +857,8 @@ __attribute__((visibility("default"))) int spinn_cuda_cache_evict(const SpinnCud
   p.budget = e->budget;
   p.recent = e->recent;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  evict_select_kernel<<<(unsigned)pairs, kSelThreads, 0, st>>>(p);
-  SPINN_CUDA_TRY(cudaGetLastError());
+  rc = launch_select(p, (int)pairs, dev, st);
+  if (rc) return rc;
   const int es = dtype_bytes(cache->dtype);
   const bool vec = cache_vec16(p.c, es);
   const int units = vec ? p.c.dim * es / 16 : p.c.dim;  // copied units of a row

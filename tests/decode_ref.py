@@ -36,10 +36,10 @@ class Paged:
 
         k, v = pool(), pool()
         for s, n in enumerate(lens):
-            for t in range(n):
-                p, o = int(table[s, t // page]), t % page
-                k[p, o] = torch.randn(kv_heads, dim, generator=g).to(dt)
-                v[p, o] = torch.randn(kv_heads, dim, generator=g).to(dt)
+            t = np.arange(n)
+            p, o = torch.from_numpy(table[s, t // page].astype(np.int64)), torch.from_numpy(t % page)
+            k[p, o] = torch.randn(n, kv_heads, dim, generator=g).to(dt)
+            v[p, o] = torch.randn(n, kv_heads, dim, generator=g).to(dt)
         self.table_host = table
 
         def put(t):  # keeps strides and offset

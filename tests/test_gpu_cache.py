@@ -264,6 +264,9 @@ EVICTS = [
     ("bf16", [3000, 1025, 7], 2, 64, 16, 1024, 100, "nhd"),
     ("fp32", [2500], 1, 4, 16, 1500, 0, "nhd"),
     ("bf16", [60, 50], 2, 256, 16, 64, 4, "nhd"),        # budget above every length
+    ("bf16", [5000, 4097, 33, 4096], 2, 8, 16, 700, 31, "nhd"),   # two CTAs to a head
+    ("fp16", [40000, 1, 20000], 1, 8, 64, 9000, 100, "nhd"),      # eight CTAs
+    ("fp16", [220000], 1, 8, 64, 5000, 0, "nhd"),                 # past the shared memory of eight
 ]
 
 
