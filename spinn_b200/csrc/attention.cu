@@ -35,6 +35,10 @@ int attention_params(const SpinnCudaCache* cache, const SpinnCudaPageTable* tabl
   SPINN_CHECK_ARG((long long)cache->kv_heads * p->gblocks <= 65535, "paged_attention: too many heads");
   p->hblocks = cache->kv_heads * p->gblocks;
   p->capacity = cache_capacity(table->max_pages, cache->page_size);
+  // (a tile holds at least 32 tokens)
+  SPINN_CHECK_ARG(((long long)p->capacity + 31) / 32 * table->seqs * p->hblocks <= kMaxUnits,
+                  "paged_attention: %d sequences of up to %d tokens in %d head blocks are too much for one call", table->seqs,
+                  p->capacity, p->hblocks);
   p->vec = cache_vec16(p->c, es);
   p->scale_log2 = a->scale * kLog2e;
   p->win = a->weights_in;
@@ -97,7 +101,7 @@ __attribute__((visibility("default"))) int spinn_cuda_paged_attention(const Spin
   if (rc) return rc;
   const AttnPlan pl = attention_plan(p, cache->dtype, sm_count(dev));
   const size_t need = pl.part + pl.ml + pl.pieces + pl.logits;
-  SPINN_CHECK_ARG(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
+  SPINN_CHECK_ARG(!need || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                   "paged_attention: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
   char* ws = static_cast<char*>(workspace);
   p.part = reinterpret_cast<float*>(ws);

@@ -13,9 +13,16 @@
 // finished there; one that crosses shares leaves a partial result per share (running maximum,
 // sum and unnormalised output), and the second kernel joins them.
 //
+// A batch whose caches are all short (the table holds at most eight tiles, and there is an SM slot
+// for every (sequence, head)) is not split: each CTA takes one (sequence, head) and there is
+// nothing to join.
+//
 // Inside a CTA the four warps take a quarter of each tile and run on their own: each has its own
-// ring of cp.async stages and its own running softmax, without a barrier in the loop, and the
-// four states are joined when a (sequence, head) ends.
+// ring of stages and its own running softmax, without a barrier in the loop, and the four states
+// are joined when a (sequence, head) ends.  Where a page holds a whole number of a warp's rows, one
+// lane fetches them with TMA boxes (two or so instructions for 4 KB, instead of a row lookup, two
+// shuffles and an address for every 512 bytes); otherwise every lane copies 16-byte pieces, or
+// single elements where rows are not aligned.
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -33,7 +40,9 @@ namespace spinn {
 namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr int kJoinWarps = 8;
+constexpr int kJoinWarps = 16;
+constexpr int kWholeTiles = 8;  // longest cache, in tiles, that is left to one CTA
+constexpr uint64_t kTimeoutNs = 4000000000ull, kDrainNs = 200000000ull;  // bounded barrier waits
 
 // Tile shapes.  GB: heads of one block (8 or 16 with 16-bit types, where they are the columns of
 // an MMA; up to 8 with fp32).  DPAD: head_dim padded to the next instantiated size.
@@ -43,17 +52,17 @@ struct Tile {
   static constexpr bool k16 = sizeof(T) == 2;
   static constexpr int RW = k16 ? 16 : 8;   // tokens of a warp
   static constexpr int TK = RW * kWarps;    // tokens of a unit
-  static constexpr int CH = DPAD * sizeof(T) / 16;
-  // Row pitch in 16-byte chunks, against bank conflicts: odd for ldmatrix (eight rows of one
-  // chunk); 4 mod 8 for the fp32 reads of two rows by four chunks.
-  static constexpr int PITCH = k16 ? CH + 1 : (CH % 8 == 4 ? CH : CH + 4);
-  static constexpr int HALF = RW * PITCH * 16;    // bytes of one warp's K (or V) rows
+  static constexpr int CH = DPAD * sizeof(T) / 16;  // 16-byte chunks of a row
+  // Rows lie in sub-tiles of 128 bytes a row, chunk c at c ^ (row % 8): the TMA's 128-byte swizzle,
+  // under which both ldmatrix and the fp32 reads are free of bank conflicts.
+  static constexpr int SUBS = CH / 8, SUB = RW * 128, HALF = SUBS * SUB;  // HALF: one warp's K (or V) rows
+  static constexpr int SPAN = 128 / sizeof(T);                            // elements of a sub-tile's row
   static constexpr int STAGE = 2 * HALF * kWarps;
   static constexpr int CPL = (CH + 31) / 32;      // fp32: float4 chunks of an output row per lane
   static constexpr int NR = k16 ? GB / 8 * (DPAD / 16) * 4 : GB * CPL * 4;  // output registers
   static constexpr int MLR = k16 ? GB / 8 * 2 : GB;  // heads whose state a lane holds
   static constexpr int DUMP = (NR + 2 * MLR) * 32 * 4;
-  static constexpr int EXTRA = 2 * DUMP + (k16 ? 0 : GB * DPAD * 4) + 2 * GB * 4 + 128;
+  static constexpr int EXTRA = 2 * DUMP + (k16 ? 0 : GB * DPAD * 4) + 2 * GB * 4 + 64 + kWarps * 6 * 8 + 16 + 1024;
   // Two CTAs per SM where three stages fit in half of the shared memory, else one
   static constexpr int kHalfSm = 113 * 1024, kSm = 226 * 1024;
   static constexpr int FIT2 = (kHalfSm - EXTRA) / STAGE, FIT1 = (kSm - EXTRA) / STAGE;
@@ -68,8 +77,9 @@ __device__ __forceinline__ float exp2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// 2^(a - b) where b is a maximum that may be -infinity (nothing seen so far).
-__device__ __forceinline__ float exp2_from(float a, float b) { return exp2_approx(a - (b == -INFINITY ? 0.0f : b)); }
+// 2^(a - b), b a reference that is finite (kNothing while nothing has been seen).
+constexpr float kNothing = -3.0e38f;
+__device__ __forceinline__ float exp2_from(float a, float b) { return exp2_approx(a - b); }
 
 __device__ __forceinline__ void cp_async_16_zfill(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -124,25 +134,19 @@ __device__ __forceinline__ T from_float(float x) {
 // (a, b) rounded to T and packed, a in the low half; lo gets what the rounding left, rounded too
 template <typename T>
 __device__ __forceinline__ uint32_t pack_split(float a, float b, uint32_t* lo) {
-  const T ha = from_float<T>(a), hb = from_float<T>(b);
-  float fa, fb;
   if constexpr (std::is_same<T, __half>::value) {
-    fa = __half2float(ha);
-    fb = __half2float(hb);
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    *lo = *reinterpret_cast<const uint32_t*>(&l);
+    return *reinterpret_cast<const uint32_t*>(&h);
   } else {
-    fa = __bfloat162float(ha);
-    fb = __bfloat162float(hb);
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(&h);
+    const __nv_bfloat162 l = __floats2bfloat162_rn(a - __uint_as_float(u << 16), b - __uint_as_float(u & 0xffff0000u));
+    *lo = *reinterpret_cast<const uint32_t*>(&l);
+    return u;
   }
-  union {
-    T t[2];
-    uint32_t u;
-  } h, l;
-  h.t[0] = ha;
-  h.t[1] = hb;
-  l.t[0] = from_float<T>(a - fa);
-  l.t[1] = from_float<T>(b - fb);
-  *lo = l.u;
-  return h.u;
 }
 
 // Length of sequence s for the launch: 0 (and the error raised) when it is out of range.
@@ -151,107 +155,159 @@ __device__ __forceinline__ int attn_len(const AttnParams& p, int s) {
   return n < 0 || n > p.capacity ? 0 : n;
 }
 
-// Position in the work: tile t of head block hb of sequence s, whose units start at `base`.
+// Position in the work: tile t of the nt tiles of head block hb of sequence s; `base` is the head
+// block's first unit.
 struct Walk {
-  long long base;
+  unsigned base;
   int s, hb, t, nt, len;
 };
+// Carries t over into the following head blocks and sequences.
+template <int TK>
+__device__ __forceinline__ void walk_carry(const AttnParams& p, Walk& w) {
+  while (w.t >= w.nt) {
+    w.t -= w.nt;
+    w.base += w.nt;
+    if (++w.hb < p.hblocks) continue;
+    w.hb = 0;
+    do {
+      ++w.s;
+      w.len = w.s < p.c.seqs ? attn_len(p, w.s) : 0x7fffffff;  // past the last: stay there
+    } while (w.len == 0);
+    w.nt = w.len == 0x7fffffff ? 0x7fffffff : (w.len + TK - 1) / TK;
+  }
+}
 template <int TK>
 __device__ __forceinline__ void walk_next(const AttnParams& p, Walk& w) {
-  if (++w.t < w.nt) return;
-  w.t = 0;
-  w.base += w.nt;  // base is the head block's first unit
-  if (++w.hb < p.hblocks) return;
-  w.hb = 0;
-  do {
-    ++w.s;
-    w.len = w.s < p.c.seqs ? attn_len(p, w.s) : 1;
-  } while (w.len == 0);
-  w.nt = (w.len + TK - 1) / TK;
+  ++w.t;
+  walk_carry<TK>(p, w);
 }
 
 template <typename T, int DPAD, int GB, bool WTS>
-__global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_kernel(const __grid_constant__ AttnParams p) {
   using C = Tile<T, DPAD, GB>;
   constexpr int TK = C::TK, RW = C::RW, NS = C::NS, NR = C::NR, MLR = C::MLR;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* dump = reinterpret_cast<float*>(smem + NS * C::STAGE);
   float* qs = dump + 2 * (C::DUMP / 4);             // fp32: [GB][DPAD] queries of the segment
   float* fin = qs + (C::k16 ? 0 : GB * DPAD);       // [2][GB] final maximum and 1 / sum (weights)
-  long long* sh = reinterpret_cast<long long*>(fin + 2 * GB);
+  unsigned* sh = reinterpret_cast<unsigned*>(fin + 2 * GB);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sh + 8);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + kWarps * 6);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint64_t* full = bars + warp * 6;  // this warp's stages
+  if (lane == 0) {
+    for (int i = 0; i < NS; ++i) mbar_init(&full[i], 1);
+    fence_mbar_init();
+  }
+  if (tid == 0) *abort_flag = 0;
   griddep_launch_dependents();
+  griddep_wait();
+  __syncthreads();
 
   // ---- this CTA's share, from the lengths
   const int workers = gridDim.x, me = blockIdx.x;
-  long long mine = 0;
-  bool bad = false;
-  for (int s = tid; s < p.c.seqs; s += kThreads) {
-    const int n = p.c.lens[s];
-    bad |= n < 0 || n > p.capacity;
-    mine += (attn_len(p, s) + TK - 1) / TK;
-  }
-  if (bad && me == 0) atomicOr(p.c.err, kCacheBadLength);
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-  if (lane == 0) sh[warp] = mine;
-  // empty sequences have no units: their outputs are zeros
-  for (int s = me; s < p.c.seqs; s += workers)
-    if (attn_len(p, s) == 0)
-      for (int i = tid; i < p.q_heads * p.c.dim; i += kThreads) {
-        const int h = i / p.c.dim;
-        static_cast<T*>(p.y)[s * p.y_seq + h * p.y_head + (i - h * p.c.dim)] = from_float<T>(0.0f);
-      }
-  __syncthreads();
-  const long long units = (sh[0] + sh[1] + sh[2] + sh[3]) * p.hblocks;
-  const long long u0 = units > 0 ? attn_start(units, workers, me) : 0;
-  const long long u1 = units > 0 ? attn_start(units, workers, me + 1) : 0;
-  if (u0 >= u1) {
-    if (tid < 2) p.pieces[me * 2 + tid].s = -1;
-    return;
-  }
-  // ---- the sequence of unit u0: scan of the tile counts, kThreads sequences at a time
+  unsigned units = 0, u0 = 0, u1 = 0;
   Walk cur;
-  {
-    long long before = 0;  // tiles of the sequences before this batch of them
-    for (int s0 = 0;; s0 += kThreads) {
-      const int s = s0 + tid;
-      const int nt = s < p.c.seqs ? (attn_len(p, s) + TK - 1) / TK : 0;
-      long long incl = nt;
+  if (p.whole) {
+    // one (sequence, head block) per CTA, its units numbered from me * whole
+    cur.s = me / p.hblocks;
+    cur.hb = me - cur.s * p.hblocks;
+    const int n = p.c.lens[cur.s];
+    if ((n < 0 || n > p.capacity) && tid == 0) atomicOr(p.c.err, kCacheBadLength);
+    cur.len = n < 0 || n > p.capacity ? 0 : n;
+    cur.nt = (cur.len + TK - 1) / TK;
+    cur.t = 0;
+    cur.base = u0 = (unsigned)me * p.whole;
+    u1 = u0 + cur.nt;
+    if (cur.len == 0) {
+      const int kvh = cur.hb / p.gblocks, g0 = (cur.hb - kvh * p.gblocks) * GB, heads = min(GB, p.group - g0);
+      T* y = static_cast<T*>(p.y) + cur.s * p.y_seq + (long long)(kvh * p.group + g0) * p.y_head;
+      for (int i = tid; i < heads * p.c.dim; i += kThreads) y[i / p.c.dim * p.y_head + i % p.c.dim] = from_float<T>(0.0f);
+      return;
+    }
+  } else {
+    // Tiles of all sequences (kThreads of them at a time), then the sequence of unit u0.  With no
+    // more sequences than threads the first scan serves for both.
+    const bool once = p.c.seqs <= kThreads;
+    unsigned total = 0, incl = 0;
+    int len = 0, nt = 0;
+    bool bad = false;
+    auto scan = [&](int s0) -> unsigned {  // inclusive over this batch, and its total
+      const int s = s0 + tid, n = s < p.c.seqs ? p.c.lens[s] : 0;
+      bad |= n < 0 || n > p.capacity;
+      len = n < 0 || n > p.capacity ? 0 : n;
+      nt = (len + TK - 1) / TK;
+      incl = nt;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
-        const long long o = __shfl_up_sync(0xffffffffu, incl, d);
+        const unsigned o = __shfl_up_sync(0xffffffffu, incl, d);
         if (lane >= d) incl += o;
       }
-      __syncthreads();
       if (lane == 31) sh[warp] = incl;
       __syncthreads();
-      for (int w = 0; w < warp; ++w) incl += sh[w];
-      const long long total = sh[0] + sh[1] + sh[2] + sh[3];
-      const long long first = (before + incl - nt) * p.hblocks;
-      if (nt > 0 && first <= u0 && u0 < first + (long long)nt * p.hblocks) {
-        sh[4] = first;
-        sh[5] = s;
+      unsigned sum = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) incl += sh[w];
+        sum += sh[w];
       }
-      before += total;
+      return sum;
+    };
+    for (int s0 = 0; s0 < p.c.seqs; s0 += kThreads) {
+      total += scan(s0);
+      if (!once) __syncthreads();
+    }
+    if (bad && me == 0) atomicOr(p.c.err, kCacheBadLength);
+    units = total * p.hblocks;
+    const AttnShares shares(units, workers);
+    u0 = shares.start(me);
+    u1 = shares.start(me + 1);
+    unsigned before = 0;  // tiles of the sequences before this batch of them
+    for (int s0 = 0; u0 < u1; s0 += kThreads) {
+      const unsigned sum = once ? total : scan(s0);
+      const unsigned first = (before + incl - nt) * p.hblocks;
+      if (nt > 0 && first <= u0 && u0 - first < (unsigned)nt * p.hblocks) {
+        sh[4] = first;
+        sh[5] = s0 + tid;
+        sh[6] = len;
+      }
+      before += sum;
+      __syncthreads();
       if (before * p.hblocks > u0) break;
     }
-    __syncthreads();
-    cur.s = (int)sh[5];
-    cur.len = attn_len(p, cur.s);
-    cur.nt = (cur.len + TK - 1) / TK;
-    const int r = (int)(u0 - sh[4]);  // < nt * hblocks; a sequence has below 2^31 of them
-    cur.hb = r / cur.nt;
-    cur.t = r - cur.hb * cur.nt;
-    cur.base = u0 - cur.t;
+    if (u0 < u1) {
+      cur.s = (int)sh[5];
+      cur.len = (int)sh[6];
+      cur.nt = (cur.len + TK - 1) / TK;
+      const unsigned r = u0 - sh[4];
+      cur.hb = (int)(r / cur.nt);
+      cur.t = (int)(r - (unsigned)cur.hb * cur.nt);
+      cur.base = u0 - cur.t;
+    }
+  }
+  // empty sequences have no units: their outputs are zeros
+  auto clear_empty = [&]() {
+    for (int s = me; s < p.c.seqs; s += workers)
+      if (attn_len(p, s) == 0)
+        for (int i = tid; i < p.q_heads * p.c.dim; i += kThreads) {
+          const int h = i / p.c.dim;
+          static_cast<T*>(p.y)[s * p.y_seq + h * p.y_head + (i - h * p.c.dim)] = from_float<T>(0.0f);
+        }
+  };
+  if (u0 >= u1) {
+    if (tid < 2) p.pieces[me * 2 + tid].s = -1;
+    clear_empty();
+    return;
   }
 
   // ---- loads: this warp's RW rows of a tile into its part of a stage
   const int count = (int)(u1 - u0);
-  const uint32_t stage0 = smem_u32(smem) + warp * 2 * C::HALF;
+  uint8_t* ring = smem + warp * 2 * C::HALF;
+  const uint32_t ring32 = smem_u32(ring);
   Walk ahead = cur;
-  // Offset of this lane's row (lanes below RW) of tile `w`, or -1 when the row is past the end
-  // or its page is bad.
+  // Lanes copying: offset of this lane's row (lanes below RW) of tile `w`, or -1 when the row is
+  // past the end or its page is bad.
   auto row_offset = [&](const Walk& w) -> long long {
     const int pos = w.t * TK + warp * RW + (lane & (RW - 1));
     if (lane >= RW || pos >= w.len) return -1;
@@ -263,10 +319,68 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
     }
     return o + (w.hb / p.gblocks) * p.c.head_stride;
   };
-  long long off = row_offset(ahead);
-  auto issue = [&](int stage) {
-    const uint32_t kdst = stage0 + stage * C::STAGE, vdst = kdst + C::HALF;
-    if (p.vec) {
+  // TMA: where the boxes of 32 tiles lie, a tile to a lane, looked up 32 tiles ahead so that no
+  // tile waits for its page number.  page -1: nothing to fetch; -2: a bad page.
+  struct Boxes {
+    int page, tok, head;
+  };
+  Boxes now = {-1, 0, 0}, next = {-1, 0, 0};
+  auto look_up = [&](int first) -> Boxes {  // tiles first .. first + 31 of this share; `ahead` is the first
+    Boxes b = {-1, 0, 0};
+    Walk w = ahead;
+    w.t += lane;
+    walk_carry<TK>(p, w);
+    const int pos = w.t * TK + warp * RW;
+    if (first + lane < count && pos < w.len) {
+      const int blk = (int)((unsigned)pos / (unsigned)p.c.page_size);
+      b.page = p.c.table[w.s * p.c.table_stride + blk];
+      b.tok = pos - blk * p.c.page_size;
+      b.head = w.hb / p.gblocks;
+      if (b.page < 0 || b.page >= p.c.num_pages) {
+        atomicOr(p.c.err, kCacheBadPage);
+        b.page = -2;
+      }
+    }
+    ahead.t += 32;
+    if (first + 32 < count) walk_carry<TK>(p, ahead);
+    return b;
+  };
+  auto chunk_at = [&](int row, int ch) -> int { return (ch >> 3) * C::SUB + row * 128 + ((ch ^ row) & 7) * 16; };
+  long long off = -1;
+  if (p.mode == kCopyTma) {
+    now = look_up(0);
+    if (count > 32) next = look_up(32);
+  } else {
+    off = row_offset(ahead);
+  }
+  auto issue = [&](int i, int stage) {  // tile i of this share
+    uint8_t* kdst = ring + stage * C::STAGE;
+    uint8_t* vdst = kdst + C::HALF;
+    if (p.mode == kCopyTma) {
+      if (i > 0 && (i & 31) == 0) {
+        now = next;
+        if (i + 32 < count) next = look_up(i + 32);
+      }
+      const int page = __shfl_sync(0xffffffffu, now.page, i & 31), tok = __shfl_sync(0xffffffffu, now.tok, i & 31);
+      const int head = __shfl_sync(0xffffffffu, now.head, i & 31);
+      if (page == -1) return;  // all of the rows are past the end: the tile is skipped
+      if (page < 0) {
+        for (int j = lane; j < 2 * C::HALF / 16; j += 32) reinterpret_cast<uint4*>(kdst)[j] = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[stage]);
+        return;
+      }
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&full[stage], 2 * C::HALF);
+        const int c1 = p.heads_inner ? head : tok, c2 = p.heads_inner ? tok : head;
+#pragma unroll
+        for (int j = 0; j < C::SUBS; ++j) {
+          tma_load_4d(&p.map_k, &full[stage], kdst + j * C::SUB, j * C::SPAN, c1, c2, page);
+          tma_load_4d(&p.map_v, &full[stage], vdst + j * C::SUB, j * C::SPAN, c1, c2, page);
+        }
+      }
+    } else if (p.mode == kCopyVec) {
       // 32 lanes cover 32 / CH rows (or a part of one row), chunk by chunk
 #pragma unroll
       for (int i = 0; i < RW * C::CH / 32; ++i) {
@@ -274,27 +388,26 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
         const long long o = __shfl_sync(0xffffffffu, off, r);
         const bool ok = o >= 0 && ch * (int)(16 / sizeof(T)) < p.c.dim;
         const long long at = ok ? o + ch * (int)(16 / sizeof(T)) : 0;
-        const uint32_t d = (r * C::PITCH + ch) * 16;
-        cp_async_16_zfill(kdst + d, static_cast<const T*>(p.c.k) + at, ok);
-        cp_async_16_zfill(vdst + d, static_cast<const T*>(p.c.v) + at, ok);
+        const int d = chunk_at(r, ch);
+        cp_async_16_zfill(smem_u32(kdst + d), static_cast<const T*>(p.c.k) + at, ok);
+        cp_async_16_zfill(smem_u32(vdst + d), static_cast<const T*>(p.c.v) + at, ok);
       }
     } else {
-      T* ks = reinterpret_cast<T*>(smem + stage * C::STAGE + warp * 2 * C::HALF);
-      T* vs = reinterpret_cast<T*>(smem + stage * C::STAGE + warp * 2 * C::HALF + C::HALF);
-      constexpr int PE = C::PITCH * 16 / sizeof(T);
+      constexpr int PER = 16 / sizeof(T);
       for (int r = 0; r < RW; ++r) {
         const long long o = __shfl_sync(0xffffffffu, off, r);
         for (int e = lane; e < DPAD; e += 32) {
           const bool ok = o >= 0 && e < p.c.dim;
-          ks[r * PE + e] = ok ? static_cast<const T*>(p.c.k)[o + e] : from_float<T>(0.0f);
-          vs[r * PE + e] = ok ? static_cast<const T*>(p.c.v)[o + e] : from_float<T>(0.0f);
+          const int d = chunk_at(r, e / PER) + e % PER * (int)sizeof(T);
+          *reinterpret_cast<T*>(kdst + d) = ok ? static_cast<const T*>(p.c.k)[o + e] : from_float<T>(0.0f);
+          *reinterpret_cast<T*>(vdst + d) = ok ? static_cast<const T*>(p.c.v)[o + e] : from_float<T>(0.0f);
         }
       }
     }
   };
-  // the next tile's table entries are read a whole tile before its rows are asked for
+  // lanes copying: the next tile's table entries are read a tile before its rows are asked for
   auto advance = [&](int issued) {
-    if (issued < count) {
+    if (p.mode != kCopyTma && issued < count) {
       walk_next<TK>(p, ahead);
       off = row_offset(ahead);
     }
@@ -302,13 +415,20 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) {
     if (i < count) {
-      issue(i);
+      issue(i, i);
       advance(i + 1);
     }
     cp_async_commit();
   }
+  uint32_t phases = 0;  // bit s: parity of the next wait for stage s
 
   // ---- running state of this warp
+  uint32_t koff[4], voff[4];  // ldmatrix addresses of the four 16-element steps of a sub-tile
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    koff[k] = (uint32_t)chunk_at(lane & 15, 2 * k + (lane >> 4));
+    voff[k] = (uint32_t)chunk_at((lane & 7) + (lane >> 4) * 8, 2 * k + ((lane >> 3) & 1));
+  }
   float o[NR / 4][4], m[MLR], l[MLR];
   uint32_t qf[C::k16 ? GB / 8 : 1][C::k16 ? DPAD / 16 : 1][2];  // 16-bit: queries as MMA fragments
   auto begin_segment = [&]() {
@@ -316,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
     for (int i = 0; i < NR; ++i) o[i / 4][i & 3] = 0.0f;
 #pragma unroll
     for (int i = 0; i < MLR; ++i) {
-      m[i] = -INFINITY;
+      m[i] = kNothing;
       l[i] = 0.0f;
     }
     const int kvh = cur.hb / p.gblocks, g0 = (cur.hb - kvh * p.gblocks) * GB;
@@ -350,68 +470,95 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
   };
 
   // ---- one tile: scores, running softmax, output
-  auto compute = [&](int stage, long long unit) {
-    const int left = cur.len - cur.t * TK - warp * RW;  // valid rows of this warp (may be <= 0)
+  auto compute = [&](int stage, unsigned unit) {
+    const int left = cur.len - cur.t * TK - warp * RW;  // valid rows of this warp
+    if (left <= 0) return;
+    uint8_t* tile = ring + stage * C::STAGE;
+    if (p.mode == kCopyTma) {
+      if (!mbar_wait(&full[stage], phases >> stage & 1, abort_flag, kTimeoutNs)) {
+        if (lane == 0) atomicOr(p.c.err, kLinearTimeout);
+      }
+      phases ^= 1u << stage;
+      if (left < RW) {
+        // what lies behind the end of the cache may be anything, and 0 * NaN is NaN
+        for (int i = lane; i < (RW - left) * C::CH; i += 32)
+          *reinterpret_cast<uint4*>(tile + C::HALF + chunk_at(left + i / C::CH, i % C::CH)) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+    }
     if constexpr (C::k16) {
       constexpr int NT = GB / 8, KD = DPAD / 16;
-      const uint32_t kb = stage0 + stage * C::STAGE, vb = kb + C::HALF;
+      const uint32_t kb = ring32 + stage * C::STAGE, vb = kb + C::HALF;
       // S^T = K Q^T: tokens are the rows, heads the columns of the MMA
       float sc[NT][2][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) sc[n][0][i] = sc[n][1][i] = 0.0f;
-      const uint32_t ka = kb + ((lane & 15) * C::PITCH + (lane >> 4)) * 16;
 #pragma unroll
       for (int k = 0; k < KD; ++k) {
         uint32_t a[4];
-        ldmatrix_x4(ka + k * 32, a);
+        ldmatrix_x4(kb + koff[k & 3] + (k >> 2) * C::SUB, a);
 #pragma unroll
         for (int n = 0; n < NT; ++n) mma_16816<T>(sc[n][k & 1], a, qf[n][k][0], qf[n][k][1]);
       }
       const int r0 = lane >> 2;
-      const bool ok0 = r0 < left, ok1 = r0 + 8 < left;
-      uint32_t ph[NT][2], pl[NT][2];
-      bool grew = false;
-      float s[NT][4], mx[MLR];
+      float t[NT][4];  // scores in log2 units, less the running reference
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[n][i] = (sc[n][0][i] + sc[n][1][i]) * p.scale_log2;
-          if (!(i < 2 ? ok0 : ok1)) s[n][i] = -INFINITY;
-        }
-        if constexpr (WTS) {
-          float* lg = p.logits + ((unit * TK + warp * RW + r0) * GB + n * 8 + (lane & 3) * 2);
-          if (ok0) *reinterpret_cast<float2*>(lg) = make_float2(s[n][0], s[n][1]);
-          if (ok1) *reinterpret_cast<float2*>(lg + 8 * GB) = make_float2(s[n][2], s[n][3]);
-        }
+        for (int i = 0; i < 4; ++i) t[n][i] = (sc[n][0][i] + sc[n][1][i]) * p.scale_log2;
+      if (left < RW) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float x = fmaxf(s[n][c], s[n][2 + c]);
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          mx[n * 2 + c] = fmaxf(x, m[n * 2 + c]);
-          grew |= mx[n * 2 + c] > m[n * 2 + c];
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (r0 + (i < 2 ? 0 : 8) >= left) t[n][i] = -INFINITY;
+      }
+      if constexpr (WTS) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int h = n * 8 + (lane & 3) * 2;
+          float* lg = p.logits + ((long long)unit * TK + warp * RW + r0) * p.lstride + h;
+          if (h < p.lstride) {
+            if (r0 < left) *reinterpret_cast<float2*>(lg) = make_float2(t[n][0], t[n][1]);
+            if (r0 + 8 < left) *reinterpret_cast<float2*>(lg + 8 * p.lstride) = make_float2(t[n][2], t[n][3]);
+          }
         }
       }
+      // The reference is raised, and what is summed so far scaled down, only when a score passes it
+      // by more than 2^8: it need not be the maximum, only keep the powers in range.
+      bool grew = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) grew |= t[n][i] - m[n * 2 + (i & 1)] > 8.0f;
       if (__any_sync(0xffffffffu, grew)) {
         float f[MLR];
 #pragma unroll
-        for (int i = 0; i < MLR; ++i) {
-          f[i] = exp2_from(m[i], mx[i]);
-          l[i] *= f[i];
-          m[i] = mx[i];
-        }
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int i = n * 2 + c;
+            float x = fmaxf(t[n][c], t[n][2 + c]);
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            x = fmaxf(x, m[i]);
+            f[i] = exp2_from(m[i], x);
+            l[i] *= f[i];
+            m[i] = x;
+          }
 #pragma unroll
         for (int i = 0; i < NR; ++i) o[i / 4][i & 3] *= f[i / (KD * 4) * 2 + (i & 1)];
       }
+      uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float e[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = exp2_from(s[n][i], m[n * 2 + (i & 1)]);
+        for (int i = 0; i < 4; ++i) e[i] = exp2_from(t[n][i], m[n * 2 + (i & 1)]);
         l[n * 2] += e[0] + e[2];
         l[n * 2 + 1] += e[1] + e[3];
         // P^T as the B operand: 8 x 8 blocks transposed in registers.  The probabilities enter
@@ -424,11 +571,10 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
         pl[n][1] = movmatrix_trans(lo1);
       }
       // O^T += V^T P^T: output dims are the rows
-      const uint32_t va = vb + (((lane & 7) + (lane >> 4) * 8) * C::PITCH + ((lane >> 3) & 1)) * 16;
 #pragma unroll
       for (int k = 0; k < KD; ++k) {
         uint32_t a[4];
-        ldmatrix_x4_trans(va + k * 32, a);
+        ldmatrix_x4_trans(vb + voff[k & 3] + (k >> 2) * C::SUB, a);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           mma_16816<T>(o[n * KD + k], a, ph[n][0], ph[n][1]);
@@ -438,8 +584,6 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
     } else {
       // fp32 on the FMA units: lane = (token of eight, quarter of the row) for the scores, a
       // chunk of four output dims for the products
-      const float4* ks = reinterpret_cast<const float4*>(smem + stage * C::STAGE + warp * 2 * C::HALF);
-      const float4* vs = ks + C::HALF / 16;
       const float4* q4 = reinterpret_cast<const float4*>(qs);
       const int key = lane >> 2, part = lane & 3;
       float s[GB];
@@ -447,10 +591,12 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
       for (int g = 0; g < GB; ++g) s[g] = 0.0f;
 #pragma unroll 4
       for (int i = 0; i < C::CH / 4; ++i) {
-        const float4 x = ks[key * C::PITCH + part + 4 * i];
+        // odd tokens take the two halves of a sub-row in the other order: all eight banks of four
+        const int ch = (i >> 1) * 8 + part + (((i ^ key) & 1) << 2);
+        const float4 x = *reinterpret_cast<const float4*>(tile + chunk_at(key, ch));
 #pragma unroll
         for (int g = 0; g < GB; ++g) {
-          const float4 y = q4[g * (DPAD / 4) + part + 4 * i];
+          const float4 y = q4[g * (DPAD / 4) + ch];
           s[g] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[g]))));
         }
       }
@@ -468,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
         mx[g] = fmaxf(x, m[g]);
         grew |= mx[g] > m[g];
         if constexpr (WTS) {
-          if (part == 0 && key < left) p.logits[(unit * TK + warp * RW + key) * GB + g] = s[g];
+          if (part == 0 && key < left && g < p.lstride) p.logits[((long long)unit * TK + warp * RW + key) * p.lstride + g] = s[g];
         }
       }
       if (__any_sync(0xffffffffu, grew)) {
@@ -491,7 +637,8 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
 #pragma unroll
         for (int ci = 0; ci < C::CPL; ++ci) {
           const int ch = lane + 32 * ci;
-          const float4 x = ch < C::CH ? vs[r * C::PITCH + ch] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          const float4 x = ch < C::CH ? *reinterpret_cast<const float4*>(tile + C::HALF + chunk_at(r, ch))
+                                      : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
           for (int g = 0; g < GB; ++g) {
             const float w = __shfl_sync(0xffffffffu, s[g], r * 4);
@@ -535,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
       o[i / 4][i & 3] = o[i / 4][i & 3] * mine[st] + d[i * 32 + lane] * other[st];
     }
   };
-  auto end_segment = [&](long long begin, long long end) {
+  auto end_segment = [&](unsigned begin, unsigned end) {
     // every lane's own share of the sum so far (16-bit: its rows; fp32: its token)
 #pragma unroll
     for (int i = 0; i < MLR; ++i) {
@@ -603,8 +750,9 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
         const int heads = p.group;  // one head block per key head with weights
         const float* win = p.win ? p.win + cur.s * p.win_seq + cur.hb * p.win_head : nullptr;
         float* wout = p.wout + cur.s * p.wout_seq + cur.hb * p.wout_head;
+#pragma unroll 2
         for (int i = tid; i < cur.len; i += kThreads) {
-          const float* lg = p.logits + (begin * TK + i) * GB;
+          const float* lg = p.logits + ((long long)begin * TK + i) * p.lstride;
           float sum = 0.0f;
           for (int g = 0; g < heads; ++g) sum += exp2_from(lg[g], fin[g]) * fin[GB + g];
           wout[i] = (win ? win[i] : 0.0f) + sum;
@@ -613,28 +761,32 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
     }
   };
 
-  if (tid < 2) p.pieces[me * 2 + tid].s = -1;
+  if (!p.whole) {
+    if (tid < 2) p.pieces[me * 2 + tid].s = -1;
+    clear_empty();
+  }
   __syncthreads();
   bool fresh = true;
   for (int i = 0; i < count; ++i) {
     if (fresh) begin_segment();
-    cp_async_wait<NS - 2>();
-    __syncwarp();  // this tile has landed, and every lane is done with the one before it
+    if (p.mode != kCopyTma) cp_async_wait<NS - 2>();
+    __syncwarp();  // every lane is done with the tile before this one (and this one's copies have landed)
     if (i + NS - 1 < count) {
-      issue((i + NS - 1) % NS);
+      issue(i + NS - 1, (i + NS - 1) % NS);
       advance(i + NS);
     }
     cp_async_commit();
     compute(i % NS, u0 + i);
     fresh = cur.t + 1 == cur.nt;
     if (fresh || i + 1 == count) {
-      const long long begin = cur.base, end = begin + cur.nt;
+      const unsigned begin = cur.base, end = begin + cur.nt;
       end_segment(begin, end);
       if (tid == 0 && (begin < u0 || end > u1)) {
         Piece& r = p.pieces[me * 2 + (begin >= u0 ? 1 : 0)];
         r.hb = cur.hb;
-        r.w0 = attn_owner(units, workers, begin);
-        r.w1 = attn_owner(units, workers, end - 1);
+        const AttnShares shares(units, workers);
+        r.w0 = shares.owner(begin);
+        r.w1 = shares.owner(end - 1);
         r.begin = begin;
         r.lo = begin >= u0 ? begin : u0;
         r.hi = end <= u1 ? end : u1;
@@ -643,97 +795,115 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
     }
     if (i + 1 < count) walk_next<TK>(p, cur);
   }
+  // after an expired wait: copies in flight land before the shared memory goes away
+  if (*abort_flag && p.mode == kCopyTma) {
+    volatile int dummy = 0;
+    for (int i = 0; i < NS; ++i) mbar_wait(&full[i], phases >> i & 1, &dummy, kDrainNs);
+  }
 }
 
 // ------------------------------------------------------------------ join
-// Block (w, slice): when worker w is the second one of a segment, the block joins four of the
-// output registers of all the segment's workers -- an online softmax over the partials, dealt to
-// eight warps.  With weights, the slices above NR / 4 turn the scores of the worker's own tokens
-// in split segments into probabilities.
+// Block (w, 0): when worker w is the second one of a segment, the block joins the partials of all
+// the segment's workers by an online softmax, four output registers to a warp, the workers dealt
+// to the warps that are left.  Blocks (w, 1 ..), with weights, turn the scores of the worker's own
+// tokens in split segments into probabilities.
 template <typename T, int DPAD, int GB, bool WTS>
-__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const AttnParams p, int weight_slices) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const __grid_constant__ AttnParams p) {
   using C = Tile<T, DPAD, GB>;
-  constexpr int TK = C::TK, NR = C::NR;
+  constexpr int TK = C::TK, NR = C::NR, SLICES = NR / 4;
+  constexpr int GROUPS = SLICES >= kJoinWarps ? 1 : kJoinWarps / SLICES;  // warps that share a slice
+  griddep_launch_dependents();
   griddep_wait();
   const int me = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if ((int)blockIdx.y < NR / 4) {
+  if (blockIdx.y == 0) {
     const Piece pc = p.pieces[me * 2];
     if (pc.s < 0) return;
     // the first worker after w0 with a share joins; workers between without one have no piece
     for (int w = pc.w0 + 1; w < me; ++w)
       if (p.pieces[w * 2].s >= 0) return;
-    __shared__ float sm[kJoinWarps][32][8];
-    const int i0 = blockIdx.y * 4;
-    int h0, h1, d[4];
-    if constexpr (C::k16) {
-      const int n = i0 / (DPAD / 16 * 4), kd = i0 / 4 % (DPAD / 16);
-      h0 = n * 8 + (lane & 3) * 2;
-      h1 = h0 + 1;
+    __shared__ float sm[GROUPS > 1 ? kJoinWarps : 1][32][9];
+    for (int slice = warp / GROUPS; slice < SLICES; slice += kJoinWarps / GROUPS) {
+      const int i0 = slice * 4;
+      int h0, h1, d[4];
+      if constexpr (C::k16) {
+        const int n = i0 / (DPAD / 16 * 4), kd = i0 / 4 % (DPAD / 16);
+        h0 = n * 8 + (lane & 3) * 2;
+        h1 = h0 + 1;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) d[i] = kd * 16 + (lane >> 2) + (i >> 1) * 8;
-    } else {
-      h0 = h1 = i0 / (C::CPL * 4);
+        for (int i = 0; i < 4; ++i) d[i] = kd * 16 + (lane >> 2) + (i >> 1) * 8;
+      } else {
+        h0 = h1 = i0 / (C::CPL * 4);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) d[i] = (lane + 32 * (i0 / 4 % C::CPL)) * 4 + i;
-    }
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int w = pc.w0 + warp; w <= pc.w1; w += kJoinWarps) {
-      const int slot = w * 2 + (w == pc.w0 ? 1 : 0);
-      if (w != pc.w0 && p.pieces[slot].s < 0) continue;
-      const float* ml = p.ml + (size_t)slot * 2 * GB;
-      const float* src = p.part + ((size_t)slot * NR + i0) * 32 + lane;
-      float x[4];
+        for (int i = 0; i < 4; ++i) d[i] = (lane + 32 * (i0 / 4 % C::CPL)) * 4 + i;
+      }
+      float m0 = kNothing, m1 = kNothing, l0 = 0.0f, l1 = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      auto add = [&](float a0, float a1, float b0, float b1, const float(&x)[4]) {
+        const float t0 = fmaxf(m0, a0), t1 = fmaxf(m1, a1);
+        const float f0 = exp2_from(m0, t0), f1 = exp2_from(m1, t1), e0 = exp2_from(a0, t0), e1 = exp2_from(a1, t1);
+        m0 = t0;
+        m1 = t1;
+        l0 = l0 * f0 + b0 * e0;
+        l1 = l1 * f1 + b1 * e1;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = src[i * 32];
-      const float a0 = ml[h0], a1 = ml[h1], b0 = ml[GB + h0], b1 = ml[GB + h1];
-      const float t0 = fmaxf(m0, a0), t1 = fmaxf(m1, a1);
-      const float f0 = exp2_from(m0, t0), f1 = exp2_from(m1, t1), e0 = exp2_from(a0, t0), e1 = exp2_from(a1, t1);
-      m0 = t0;
-      m1 = t1;
-      l0 = l0 * f0 + b0 * e0;
-      l1 = l1 * f1 + b1 * e1;
+        for (int i = 0; i < 4; ++i) o[i] = C::k16 && (i & 1) ? o[i] * f1 + x[i] * e1 : o[i] * f0 + x[i] * e0;
+      };
+      constexpr int U = 4;  // partials in flight
+      for (int wb = pc.w0 + warp % GROUPS; wb <= pc.w1; wb += U * GROUPS) {
+        float x[U][4], a0[U], a1[U], b0[U], b1[U];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = C::k16 && (i & 1) ? o[i] * f1 + x[i] * e1 : o[i] * f0 + x[i] * e0;
-    }
-    float* mine = sm[warp][lane];
-    mine[0] = m0;
-    mine[1] = m1;
-    mine[2] = l0;
-    mine[3] = l1;
+        for (int u = 0; u < U; ++u) {
+          const int w = wb + u * GROUPS, slot = w * 2 + (w == pc.w0 ? 1 : 0);
+          a0[u] = a1[u] = kNothing;
+          b0[u] = b1[u] = x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.0f;
+          if (w > pc.w1 || (w != pc.w0 && p.pieces[slot].s < 0)) continue;
+          const float* ml = p.ml + (size_t)slot * 2 * GB;
+          const float* src = p.part + ((size_t)slot * NR + i0) * 32 + lane;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mine[4 + i] = o[i];
-    __syncthreads();
-    if (warp != 0) return;
-    for (int w = 1; w < kJoinWarps; ++w) {
-      const float* x = sm[w][lane];
-      const float t0 = fmaxf(m0, x[0]), t1 = fmaxf(m1, x[1]);
-      const float f0 = exp2_from(m0, t0), f1 = exp2_from(m1, t1), e0 = exp2_from(x[0], t0), e1 = exp2_from(x[1], t1);
-      m0 = t0;
-      m1 = t1;
-      l0 = l0 * f0 + x[2] * e0;
-      l1 = l1 * f1 + x[3] * e1;
+          for (int i = 0; i < 4; ++i) x[u][i] = src[i * 32];
+          a0[u] = ml[h0];
+          a1[u] = ml[h1];
+          b0[u] = ml[GB + h0];
+          b1[u] = ml[GB + h1];
+        }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = C::k16 && (i & 1) ? o[i] * f1 + x[4 + i] * e1 : o[i] * f0 + x[4 + i] * e0;
-    }
-    const int kvh = pc.hb / p.gblocks, g0 = (pc.hb - kvh * p.gblocks) * GB;
-    const int heads = min(GB, p.group - g0);
-    T* y = static_cast<T*>(p.y) + pc.s * p.y_seq + (long long)(kvh * p.group + g0) * p.y_head;
+        for (int u = 0; u < U; ++u) add(a0[u], a1[u], b0[u], b1[u], x[u]);
+      }
+      if constexpr (GROUPS > 1) {
+        float* mine = sm[warp][lane];
+        mine[0] = m0;
+        mine[1] = m1;
+        mine[2] = l0;
+        mine[3] = l1;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int h = C::k16 && (i & 1) ? h1 : h0;
-      if (h < heads && d[i] < p.c.dim) y[h * p.y_head + d[i]] = from_float<T>(o[i] / (C::k16 && (i & 1) ? l1 : l0));
+        for (int i = 0; i < 4; ++i) mine[4 + i] = o[i];
+        __syncthreads();
+        if (warp % GROUPS) return;
+        for (int w = warp + 1; w < warp + GROUPS; ++w) {
+          const float* x = sm[w][lane];
+          const float xo[4] = {x[4], x[5], x[6], x[7]};
+          add(x[0], x[1], x[2], x[3], xo);
+        }
+      }
+      const int kvh = pc.hb / p.gblocks, g0 = (pc.hb - kvh * p.gblocks) * GB;
+      const int heads = min(GB, p.group - g0);
+      T* y = static_cast<T*>(p.y) + pc.s * p.y_seq + (long long)(kvh * p.group + g0) * p.y_head;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int h = C::k16 && (i & 1) ? h1 : h0;
+        if (h < heads && d[i] < p.c.dim) y[h * p.y_head + d[i]] = from_float<T>(o[i] / (C::k16 && (i & 1) ? l1 : l0));
+      }
     }
     return;
   }
   if constexpr (WTS) {
     __shared__ float top[GB], inv[GB];
-    const int slice = blockIdx.y - NR / 4;
+    const int slice = blockIdx.y - 1, slices = gridDim.y - 1;
     for (int kind = 0; kind < 2; ++kind) {
       const Piece pc = p.pieces[me * 2 + kind];
       if (pc.s < 0) continue;
       const int len = p.c.lens[pc.s];
       for (int g = warp; g < p.group; g += kJoinWarps) {
-        float m = -INFINITY, l = 0.0f;
+        float m = kNothing, l = 0.0f;
         for (int w = pc.w0 + lane; w <= pc.w1; w += 32) {
           const int slot = w * 2 + (w == pc.w0 ? 1 : 0);
           if (w != pc.w0 && p.pieces[slot].s < 0) continue;
@@ -759,42 +929,96 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const A
       float* wout = p.wout + pc.s * p.wout_seq + pc.hb * p.wout_head;
       // this worker's tokens of the segment, dealt to the slices
       const int t0 = (int)(pc.lo - pc.begin) * TK, t1 = min(len, (int)(pc.hi - pc.begin) * TK);
-      for (int i = t0 + slice * kJoinWarps * 32 + tid; i < t1; i += weight_slices * kJoinWarps * 32) {
-        const float* lg = p.logits + (pc.begin * TK + i) * GB;
-        float sum = 0.0f;
-        for (int g = 0; g < p.group; ++g) sum += exp2_from(lg[g], top[g]) * inv[g];
-        wout[i] = (win ? win[i] : 0.0f) + sum;
+      constexpr int U = 4;  // tokens of a thread in flight
+      const int step = slices * kJoinWarps * 32;
+      for (int i0 = t0 + slice * kJoinWarps * 32 + tid; i0 < t1; i0 += U * step) {
+        float w[U], sum[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int i = i0 + u * step;
+          w[u] = win && i < t1 ? win[i] : 0.0f;
+          sum[u] = 0.0f;
+        }
+        const float* lg = p.logits + ((long long)pc.begin * TK + i0) * p.lstride;
+        const long long lstep = (long long)step * p.lstride;
+        if (C::k16) {  // an even number of scores per token
+          for (int g = 0; g < p.lstride; g += 2) {
+            float2 x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+              x[u] = i0 + u * step < t1 ? *reinterpret_cast<const float2*>(lg + u * lstep + g) : make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              sum[u] += exp2_from(x[u].x, top[g]) * inv[g];
+              if (g + 1 < p.group) sum[u] += exp2_from(x[u].y, top[g + 1]) * inv[g + 1];
+            }
+          }
+        } else {
+          for (int g = 0; g < p.group; ++g)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+              if (i0 + u * step < t1) sum[u] += exp2_from(lg[u * lstep + g], top[g]) * inv[g];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (i0 + u * step < t1) wout[i0 + u * step] = w[u] + sum[u];
       }
       __syncthreads();
     }
   }
 }
 
-// Workspace of a launch (bytes of its parts, each rounded to 256).
+// CTAs of a launch and the bytes of the parts of its workspace.
 template <typename T, int DPAD, int GB>
 AttnPlan attention_plan_for(const AttnParams& p, int sms, bool weights) {
   using C = Tile<T, DPAD, GB>;
   const long long tiles = ((long long)p.capacity + C::TK - 1) / C::TK;
-  const long long units = tiles * p.c.seqs * p.hblocks;  // at most
+  const long long segments = (long long)p.c.seqs * p.hblocks, units = tiles * segments;  // at most
   AttnPlan pl;
-  pl.workers = (int)std::min<long long>(units, (long long)sms * C::CTAS);
-  pl.part = up256((size_t)pl.workers * 2 * C::NR * 32 * 4);
-  pl.ml = up256((size_t)pl.workers * 2 * 2 * GB * 4);
-  pl.pieces = up256((size_t)pl.workers * 2 * sizeof(Piece));
-  pl.logits = weights ? up256((size_t)units * C::TK * GB * 4) : 0;
+  // Short caches, a CTA each: the join costs more than the few tiles in a row (333 tokens, 4
+  // heads of 64: 10.2 us split, XX whole)
+  pl.whole = tiles <= kWholeTiles && segments <= (long long)sms * C::CTAS;
+  pl.workers = pl.whole ? (int)segments : (int)std::min<long long>(units, (long long)sms * C::CTAS);
+  pl.part = pl.whole ? 0 : up256((size_t)pl.workers * 2 * C::NR * 32 * 4);
+  pl.ml = pl.whole ? 0 : up256((size_t)pl.workers * 2 * 2 * GB * 4);
+  pl.pieces = pl.whole ? 0 : up256((size_t)pl.workers * 2 * sizeof(Piece));
+  pl.lstride = C::k16 ? (p.group + 1) / 2 * 2 : p.group;
+  pl.logits = weights ? up256((size_t)units * C::TK * pl.lstride * 4) : 0;
   return pl;
 }
 
+// Tensor maps of the pools for boxes of a warp's rows of one head, when their layout allows: false
+// leaves the copies to the lanes.
+template <typename C, typename T>
+bool attention_maps(AttnParams* p) {
+  const CacheView& c = p->c;
+  if (!p->vec || c.page_size % C::RW) return false;
+  const long long tok = c.token_stride, head = c.head_stride;
+  p->heads_inner = head <= tok;
+  const long long in = p->heads_inner ? head : tok, out = p->heads_inner ? tok : head;
+  if (in <= 0 || out % in || c.page_stride < out || c.page_stride % out) return false;
+  const int n_in = p->heads_inner ? c.kv_heads : c.page_size, n_out = p->heads_inner ? c.page_size : c.kv_heads;
+  const int b_in = p->heads_inner ? 1 : C::RW, b_out = p->heads_inner ? C::RW : 1;
+  const uint64_t dims[4] = {(uint64_t)c.dim, (uint64_t)n_in, (uint64_t)n_out, (uint64_t)c.num_pages};
+  const uint64_t strides[3] = {(uint64_t)in * sizeof(T), (uint64_t)out * sizeof(T), (uint64_t)c.page_stride * sizeof(T)};
+  const uint32_t box[4] = {(uint32_t)C::SPAN, (uint32_t)b_in, (uint32_t)b_out, 1};
+  if (c.dim < 16 / (int)sizeof(T) || strides[2] >= (1ull << 40)) return false;
+  return encode_tiled_4d_sw128(&p->map_k, c.k, sizeof(T), dims, strides, box) == 0 &&
+         encode_tiled_4d_sw128(&p->map_v, c.v, sizeof(T), dims, strides, box) == 0;
+}
+
 template <typename T, int DPAD, int GB, bool WTS>
-int attention_launch_for(const AttnParams& p, const AttnPlan& pl, cudaStream_t st) {
+int attention_launch_for(AttnParams& p, const AttnPlan& pl, cudaStream_t st) {
   using C = Tile<T, DPAD, GB>;
+  p.mode = attention_maps<C, T>(&p) ? kCopyTma : p.vec ? kCopyVec : kCopyElements;
+  p.whole = pl.whole ? (p.capacity + C::TK - 1) / C::TK : 0;
+  p.lstride = pl.lstride;
   auto* kernel = attention_kernel<T, DPAD, GB, WTS>;
   SPINN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-  kernel<<<pl.workers, kThreads, C::SMEM, st>>>(p);
-  SPINN_CUDA_TRY(cudaGetLastError());
-  const int slices = WTS ? 4 : 0;
-  return launch_dependent(attention_join_kernel<T, DPAD, GB, WTS>, dim3(pl.workers, C::NR / 4 + slices), kJoinWarps * 32,
-                          0, st, p, slices);
+  const int rc = launch_dependent(kernel, dim3(pl.workers), kThreads, C::SMEM, st, p);
+  if (rc || pl.whole) return rc;
+  return launch_dependent(attention_join_kernel<T, DPAD, GB, WTS>, dim3(pl.workers, WTS ? 3 : 1), kJoinWarps * 32, 0, st,
+                          p);
 }
 
 // The instantiation for a head size and group: `go` gets the Tile as a tag.
@@ -819,7 +1043,7 @@ AttnPlan attention_plan_t(const AttnParams& p, int sms, bool weights) {
   });
 }
 template <typename T>
-int attention_launch_t(const AttnParams& p, const AttnPlan& pl, cudaStream_t st) {
+int attention_launch_t(AttnParams& p, const AttnPlan& pl, cudaStream_t st) {
   return attention_dispatch<T>(p.c.dim, p.group, [&](auto t) {
     using C = decltype(t);
     return p.wout ? attention_launch_for<T, C::DPAD, C::GB, true>(p, pl, st)

@@ -1,6 +1,8 @@
 // attention.h -- parameters of the paged attention launch (attention.cuh), and the instantiations
 // for each cache type, one translation unit each.
 #pragma once
+#include <cuda.h>
+
 #include "cache.h"
 
 namespace spinn {
@@ -12,17 +14,24 @@ namespace spinn {
 struct Piece {
   int s, hb;  // s < 0: none
   int w0, w1;
-  long long begin, lo, hi;
+  unsigned begin, lo, hi;
 };
 
+enum AttnCopy { kCopyElements = 0, kCopyVec = 1, kCopyTma = 2 };
+
 struct AttnParams {
+  CUtensorMap map_k, map_v;  // kCopyTma: boxes of a warp's rows of one head
   CacheView c;
   const void* q;
   void* y;
   long long q_seq, q_head, y_seq, y_head;
   int q_heads, group, gblocks, hblocks;  // hblocks = kv_heads * gblocks
   int capacity;                          // longest allowed length
-  bool vec;                              // 16-byte loads of the cache
+  bool vec;                              // 16-byte rows
+  bool heads_inner;                      // the maps' second dimension is the head, not the token
+  int mode;                              // AttnCopy
+  int whole;                             // tiles to number per CTA when nothing is split, else 0
+  int lstride;                           // scores kept per token (weights only)
   float scale_log2;
   const float* win;
   float* wout;
@@ -30,12 +39,13 @@ struct AttnParams {
   float* part;    // [worker][2][NR * 32] unnormalised outputs, in register order
   float* ml;      // [worker][2][2][GB] maxima and sums
   Piece* pieces;  // [worker][2]
-  float* logits;  // [unit][TK][GB], scores in log2 units (weights only)
+  float* logits;  // [unit][TK][lstride], scores in log2 units (weights only)
 };
 
 // CTAs of a launch and the bytes of each part of its workspace.
 struct AttnPlan {
-  int workers;
+  bool whole;  // one CTA per (sequence, head block), nothing to join
+  int workers, lstride;
   size_t part, ml, pieces, logits;
 };
 
@@ -50,8 +60,8 @@ inline int attention_head_block(int bytes, int group) {
 AttnPlan attention_plan_fp16(const AttnParams& p, int sms, bool weights);
 AttnPlan attention_plan_bf16(const AttnParams& p, int sms, bool weights);
 AttnPlan attention_plan_fp32(const AttnParams& p, int sms, bool weights);
-int attention_launch_fp16(const AttnParams& p, const AttnPlan& pl, cudaStream_t st);
-int attention_launch_bf16(const AttnParams& p, const AttnPlan& pl, cudaStream_t st);
-int attention_launch_fp32(const AttnParams& p, const AttnPlan& pl, cudaStream_t st);
+int attention_launch_fp16(AttnParams& p, const AttnPlan& pl, cudaStream_t st);
+int attention_launch_bf16(AttnParams& p, const AttnPlan& pl, cudaStream_t st);
+int attention_launch_fp32(AttnParams& p, const AttnPlan& pl, cudaStream_t st);
 
 }  // namespace spinn

@@ -6,7 +6,7 @@ namespace spinn {
 AttnPlan attention_plan_bf16(const AttnParams& p, int sms, bool weights) {
   return attention_plan_t<__nv_bfloat16>(p, sms, weights);
 }
-int attention_launch_bf16(const AttnParams& p, const AttnPlan& pl, cudaStream_t st) {
+int attention_launch_bf16(AttnParams& p, const AttnPlan& pl, cudaStream_t st) {
   return attention_launch_t<__nv_bfloat16>(p, pl, st);
 }
 

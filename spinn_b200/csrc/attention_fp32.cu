@@ -6,7 +6,7 @@ namespace spinn {
 AttnPlan attention_plan_fp32(const AttnParams& p, int sms, bool weights) {
   return attention_plan_t<float>(p, sms, weights);
 }
-int attention_launch_fp32(const AttnParams& p, const AttnPlan& pl, cudaStream_t st) {
+int attention_launch_fp32(AttnParams& p, const AttnPlan& pl, cudaStream_t st) {
   return attention_launch_t<float>(p, pl, st);
 }
 

@@ -888,11 +888,13 @@ __attribute__((visibility("default"))) int64_t spinn_cuda_diag_cache_slot(const 
 
 __attribute__((visibility("default"))) int spinn_cuda_diag_attention_share(int64_t units, int workers, int worker,
                                                                            int64_t unit, int64_t* out3) {
-  SPINN_CHECK_ARG(out3 && units > 0 && workers > 0 && worker >= 0 && worker < workers && unit >= 0 && unit < units,
+  SPINN_CHECK_ARG(out3 && units > 0 && units <= kMaxUnits && workers > 0 && worker >= 0 && worker < workers && unit >= 0 &&
+                      unit < units,
                   "spinn_cuda_diag_attention_share: invalid arguments");
-  out3[0] = attn_start(units, workers, worker);
-  out3[1] = attn_start(units, workers, worker + 1);
-  out3[2] = attn_owner(units, workers, unit);
+  const AttnShares sh((unsigned)units, (unsigned)workers);
+  out3[0] = sh.start((unsigned)worker);
+  out3[1] = sh.start((unsigned)worker + 1);
+  out3[2] = sh.owner((unsigned)unit);
   return 0;
 }
 

@@ -45,15 +45,18 @@ __host__ __device__ inline long long cache_slot(const int* row, int pos, int pag
 }
 
 // Attention's work: `units` tiles of tokens in the order (sequence, head block, tile), dealt to
-// `workers` CTAs in equal contiguous shares.  Worker w has [attn_start(w), attn_start(w + 1)).
-__host__ __device__ inline long long attn_start(long long units, int workers, int w) {
-  return units * w / workers;
-}
-// The worker whose share holds unit u: the last w with floor(units * w / workers) <= u, i.e. the
-// last w below (u + 1) * workers / units.
-__host__ __device__ inline int attn_owner(long long units, int workers, long long u) {
-  return (int)(((u + 1) * workers + units - 1) / units) - 1;
-}
+// `workers` CTAs in contiguous shares of units / workers, the first units % workers of them one
+// more.  Worker w has [start(w), start(w + 1)); owner(u) is the worker that has unit u.
+struct AttnShares {
+  unsigned each, more;
+  __host__ __device__ AttnShares(unsigned units, unsigned workers) : each(units / workers), more(units - each * workers) {}
+  __host__ __device__ unsigned start(unsigned w) const { return w * each + (w < more ? w : more); }
+  __host__ __device__ int owner(unsigned u) const {
+    const unsigned big = more * (each + 1);
+    return (int)(u < big ? u / (each + 1) : more + (u - big) / each);
+  }
+};
+constexpr long long kMaxUnits = 0x7fffffffLL;
 
 // Host-side checks common to the cache entry points; fills `v`.
 int cache_view(const char* who, const SpinnCudaCache* c, const SpinnCudaPageTable* t, CacheView* v);
