@@ -200,7 +200,13 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
     for (int i = 0; i < NS; ++i) mbar_init(&full[i], 1);
     fence_mbar_init();
   }
-  if (tid == 0) *abort_flag = 0;
+  if (tid == 0) {
+    *abort_flag = 0;
+    if (p.mode == kCopyTma) {
+      prefetch_tmap(&p.map_k);
+      prefetch_tmap(&p.map_v);
+    }
+  }
   griddep_launch_dependents();
   griddep_wait();
   __syncthreads();
@@ -324,6 +330,15 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
   struct Boxes {
     int page, tok, head;
   };
+  // sub-tiles past head_dim are never fetched: they stay the zeros they are made here
+  const int boxes = (p.c.dim + C::SPAN - 1) / C::SPAN;
+  if (p.mode == kCopyTma && boxes < C::SUBS) {
+    for (int i = 0; i < NS; ++i)
+      for (int h = 0; h < 2; ++h)
+        for (int j = boxes * (C::SUB / 16) + lane; j < C::HALF / 16; j += 32)
+          *reinterpret_cast<uint4*>(ring + i * C::STAGE + h * C::HALF + j * 16) = make_uint4(0, 0, 0, 0);
+    __syncwarp();
+  }
   Boxes now = {-1, 0, 0}, next = {-1, 0, 0};
   auto look_up = [&](int first) -> Boxes {  // tiles first .. first + 31 of this share; `ahead` is the first
     Boxes b = {-1, 0, 0};
@@ -372,10 +387,11 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
         return;
       }
       if (lane == 0) {
-        mbar_arrive_expect_tx(&full[stage], 2 * C::HALF);
+        mbar_arrive_expect_tx(&full[stage], 2 * boxes * C::SUB);
         const int c1 = p.heads_inner ? head : tok, c2 = p.heads_inner ? tok : head;
 #pragma unroll
         for (int j = 0; j < C::SUBS; ++j) {
+          if (j >= boxes) break;
           tma_load_4d(&p.map_k, &full[stage], kdst + j * C::SUB, j * C::SPAN, c1, c2, page);
           tma_load_4d(&p.map_v, &full[stage], vdst + j * C::SUB, j * C::SPAN, c1, c2, page);
         }
@@ -589,8 +605,9 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
       float s[GB];
 #pragma unroll
       for (int g = 0; g < GB; ++g) s[g] = 0.0f;
+      const int chunks = (p.c.dim + 31) / 32 * 2;  // pairs of steps that hold head_dim
 #pragma unroll 4
-      for (int i = 0; i < C::CH / 4; ++i) {
+      for (int i = 0; i < chunks; ++i) {
         // odd tokens take the two halves of a sub-row in the other order: all eight banks of four
         const int ch = (i >> 1) * 8 + part + (((i ^ key) & 1) << 2);
         const float4 x = *reinterpret_cast<const float4*>(tile + chunk_at(key, ch));
@@ -601,28 +618,27 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
         }
       }
       bool grew = false;
-      float mx[GB];
 #pragma unroll
       for (int g = 0; g < GB; ++g) {
         s[g] += __shfl_xor_sync(0xffffffffu, s[g], 1);
         s[g] += __shfl_xor_sync(0xffffffffu, s[g], 2);
         s[g] = key < left ? s[g] * p.scale_log2 : -INFINITY;
-        float x = s[g];
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-        mx[g] = fmaxf(x, m[g]);
-        grew |= mx[g] > m[g];
+        grew |= s[g] - m[g] > 8.0f;
         if constexpr (WTS) {
           if (part == 0 && key < left && g < p.lstride) p.logits[((long long)unit * TK + warp * RW + key) * p.lstride + g] = s[g];
         }
       }
-      if (__any_sync(0xffffffffu, grew)) {
+      if (__any_sync(0xffffffffu, grew)) {  // as above
 #pragma unroll
         for (int g = 0; g < GB; ++g) {
-          const float f = exp2_from(m[g], mx[g]);
+          float x = s[g];
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          x = fmaxf(x, m[g]);
+          const float f = exp2_from(m[g], x);
           l[g] *= f;
-          m[g] = mx[g];
+          m[g] = x;
 #pragma unroll
           for (int i = 0; i < C::CPL * 4; ++i) o[g * C::CPL + i / 4][i & 3] *= f;
         }
