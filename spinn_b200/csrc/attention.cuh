@@ -53,10 +53,10 @@ struct Tile {
   static constexpr int RW = k16 ? 16 : 8;   // tokens of a warp
   static constexpr int TK = RW * kWarps;    // tokens of a unit
   static constexpr int CH = DPAD * sizeof(T) / 16;  // 16-byte chunks of a row
-  // Rows lie in sub-tiles of 128 bytes a row, chunk c at c ^ (row % 8): the TMA's 128-byte swizzle,
-  // under which both ldmatrix and the fp32 reads are free of bank conflicts.
-  static constexpr int SUBS = CH / 8, SUB = RW * 128, HALF = SUBS * SUB;  // HALF: one warp's K (or V) rows
-  static constexpr int SPAN = 128 / sizeof(T);                            // elements of a sub-tile's row
+  // 16-bit rows lie in sub-tiles of 128 bytes a row, chunk c at c ^ (row % 8): the TMA's 128-byte
+  // swizzle, under which ldmatrix is free of bank conflicts.  fp32 rows lie one behind the other.
+  static constexpr int SUBS = CH / 8, SUB = RW * 128, HALF = RW * CH * 16;  // HALF: one warp's K (or V) rows
+  static constexpr int SPAN = k16 ? 64 : 0;                                 // elements of a sub-tile's row
   static constexpr int STAGE = 2 * HALF * kWarps;
   static constexpr int CPL = (CH + 31) / 32;      // fp32: float4 chunks of an output row per lane
   static constexpr int NR = k16 ? GB / 8 * (DPAD / 16) * 4 : GB * CPL * 4;  // output registers
@@ -311,6 +311,11 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
   const int count = (int)(u1 - u0);
   uint8_t* ring = smem + warp * 2 * C::HALF;
   const uint32_t ring32 = smem_u32(ring);
+  // fp32: bytes from row to row, which a box of whole rows lays end to end
+  const int pitch = p.mode == kCopyTma ? p.c.dim * 4 : DPAD * 4;
+  auto chunk_at = [&](int row, int ch) -> int {
+    return C::k16 ? (ch >> 3) * C::SUB + row * 128 + ((ch ^ row) & 7) * 16 : row * pitch + ch * 16;
+  };
   Walk ahead = cur;
   // Lanes copying: offset of this lane's row (lanes below RW) of tile `w`, or -1 when the row is
   // past the end or its page is bad.
@@ -331,8 +336,9 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
     int page, tok, head;
   };
   // sub-tiles past head_dim are never fetched: they stay the zeros they are made here
-  const int boxes = (p.c.dim + C::SPAN - 1) / C::SPAN;
-  if (p.mode == kCopyTma && boxes < C::SUBS) {
+  const int boxes = C::k16 ? (p.c.dim + 63) / 64 : 1;
+  const uint32_t fetched = C::k16 ? 2 * boxes * C::SUB : 2 * RW * pitch;  // bytes of a warp's tile
+  if (C::k16 && p.mode == kCopyTma && boxes < C::SUBS) {
     for (int i = 0; i < NS; ++i)
       for (int h = 0; h < 2; ++h)
         for (int j = boxes * (C::SUB / 16) + lane; j < C::HALF / 16; j += 32)
@@ -360,7 +366,6 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
     if (first + 32 < count) walk_carry<TK>(p, ahead);
     return b;
   };
-  auto chunk_at = [&](int row, int ch) -> int { return (ch >> 3) * C::SUB + row * 128 + ((ch ^ row) & 7) * 16; };
   long long off = -1;
   if (p.mode == kCopyTma) {
     now = look_up(0);
@@ -387,10 +392,10 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
         return;
       }
       if (lane == 0) {
-        mbar_arrive_expect_tx(&full[stage], 2 * boxes * C::SUB);
+        mbar_arrive_expect_tx(&full[stage], fetched);
         const int c1 = p.heads_inner ? head : tok, c2 = p.heads_inner ? tok : head;
 #pragma unroll
-        for (int j = 0; j < C::SUBS; ++j) {
+        for (int j = 0; j < (C::k16 ? C::SUBS : 1); ++j) {
           if (j >= boxes) break;
           tma_load_4d(&p.map_k, &full[stage], kdst + j * C::SUB, j * C::SPAN, c1, c2, page);
           tma_load_4d(&p.map_v, &full[stage], vdst + j * C::SUB, j * C::SPAN, c1, c2, page);
@@ -497,8 +502,13 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
       phases ^= 1u << stage;
       if (left < RW) {
         // what lies behind the end of the cache may be anything, and 0 * NaN is NaN
-        for (int i = lane; i < (RW - left) * C::CH; i += 32)
-          *reinterpret_cast<uint4*>(tile + C::HALF + chunk_at(left + i / C::CH, i % C::CH)) = make_uint4(0, 0, 0, 0);
+        if constexpr (C::k16) {
+          for (int i = lane; i < (RW - left) * C::CH; i += 32)
+            *reinterpret_cast<uint4*>(tile + C::HALF + chunk_at(left + i / C::CH, i % C::CH)) = make_uint4(0, 0, 0, 0);
+        } else {
+          for (int i = left * pitch + lane * 16; i < RW * pitch; i += 512)
+            *reinterpret_cast<uint4*>(tile + C::HALF + i) = make_uint4(0, 0, 0, 0);
+        }
         fence_proxy_async_smem();
         __syncwarp();
       }
@@ -605,11 +615,14 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
       float s[GB];
 #pragma unroll
       for (int g = 0; g < GB; ++g) s[g] = 0.0f;
-      const int chunks = (p.c.dim + 31) / 32 * 2;  // pairs of steps that hold head_dim
+      // Four lanes to a token take every fourth chunk.  Where rows start on the same banks, odd tokens
+      // take the chunks of a pair of steps in the other order: all eight groups of banks at once.
+      const int chunks = (p.c.dim + 3) >> 2;
+      const int flip = pitch % 128 == 0 ? (key & 1) << 2 : 0;
 #pragma unroll 4
-      for (int i = 0; i < chunks; ++i) {
-        // odd tokens take the two halves of a sub-row in the other order: all eight banks of four
-        const int ch = (i >> 1) * 8 + part + (((i ^ key) & 1) << 2);
+      for (int i = 0; i < chunks; i += 4) {
+        const int ch = i + part < chunks && (i ^ flip) + part < chunks ? (i ^ flip) + part : i + part;
+        if (ch >= chunks) continue;
         const float4 x = *reinterpret_cast<const float4*>(tile + chunk_at(key, ch));
 #pragma unroll
         for (int g = 0; g < GB; ++g) {
@@ -653,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
 #pragma unroll
         for (int ci = 0; ci < C::CPL; ++ci) {
           const int ch = lane + 32 * ci;
-          const float4 x = ch < C::CH ? *reinterpret_cast<const float4*>(tile + C::HALF + chunk_at(r, ch))
+          const float4 x = ch < (p.c.dim + 3) >> 2 ? *reinterpret_cast<const float4*>(tile + C::HALF + chunk_at(r, ch))
                                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
           for (int g = 0; g < GB; ++g) {
@@ -1017,10 +1030,10 @@ bool attention_maps(AttnParams* p) {
   const int b_in = p->heads_inner ? 1 : C::RW, b_out = p->heads_inner ? C::RW : 1;
   const uint64_t dims[4] = {(uint64_t)c.dim, (uint64_t)n_in, (uint64_t)n_out, (uint64_t)c.num_pages};
   const uint64_t strides[3] = {(uint64_t)in * sizeof(T), (uint64_t)out * sizeof(T), (uint64_t)c.page_stride * sizeof(T)};
-  const uint32_t box[4] = {(uint32_t)C::SPAN, (uint32_t)b_in, (uint32_t)b_out, 1};
+  const uint32_t box[4] = {C::k16 ? 64u : (uint32_t)c.dim, (uint32_t)b_in, (uint32_t)b_out, 1};
   if (c.dim < 16 / (int)sizeof(T) || strides[2] >= (1ull << 40)) return false;
-  return encode_tiled_4d_sw128(&p->map_k, c.k, sizeof(T), dims, strides, box) == 0 &&
-         encode_tiled_4d_sw128(&p->map_v, c.v, sizeof(T), dims, strides, box) == 0;
+  return encode_tiled_4d(&p->map_k, c.k, sizeof(T), dims, strides, box) == 0 &&
+         encode_tiled_4d(&p->map_v, c.v, sizeof(T), dims, strides, box) == 0;
 }
 
 template <typename T, int DPAD, int GB, bool WTS>
@@ -1033,7 +1046,7 @@ int attention_launch_for(AttnParams& p, const AttnPlan& pl, cudaStream_t st) {
   SPINN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
   const int rc = launch_dependent(kernel, dim3(pl.workers), kThreads, C::SMEM, st, p);
   if (rc || pl.whole) return rc;
-  return launch_dependent(attention_join_kernel<T, DPAD, GB, WTS>, dim3(pl.workers, WTS ? 3 : 1), kJoinWarps * 32, 0, st,
+  return launch_dependent(attention_join_kernel<T, DPAD, GB, WTS>, dim3(pl.workers, WTS ? 2 : 1), kJoinWarps * 32, 0, st,
                           p);
 }
 

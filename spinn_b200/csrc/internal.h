@@ -43,9 +43,9 @@ int encode_tiled_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t
 // The same for 16-bit elements (128-byte swizzle).
 int encode_tiled_2d_16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
                        uint32_t box_inner, uint32_t box_outer, bool fp16);
-// 4-D tiled map with 128-byte swizzle of 16- or 32-bit elements (strides in bytes, rising).
-int encode_tiled_4d_sw128(CUtensorMap* map, const void* base, int element_bytes, const uint64_t (&dims)[4],
-                          const uint64_t (&strides)[3], const uint32_t (&box)[4]);
+// 4-D tiled map of 16-bit (128-byte swizzle) or 32-bit (no swizzle) elements, strides in bytes, rising.
+int encode_tiled_4d(CUtensorMap* map, const void* base, int element_bytes, const uint64_t (&dims)[4],
+                    const uint64_t (&strides)[3], const uint32_t (&box)[4]);
 // 3-D tiled map of `planes` row-major [outer][inner] matrices stored back to back.
 int encode_tiled_3d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t planes,
                     uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle);

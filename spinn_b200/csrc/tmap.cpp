@@ -109,8 +109,8 @@ int encode_tiled_2d_16(CUtensorMap* map, const void* base, uint64_t inner, uint6
   return 0;
 }
 
-int encode_tiled_4d_sw128(CUtensorMap* map, const void* base, int element_bytes, const uint64_t (&dims)[4],
-                          const uint64_t (&strides)[3], const uint32_t (&box)[4]) {
+int encode_tiled_4d(CUtensorMap* map, const void* base, int element_bytes, const uint64_t (&dims)[4],
+                    const uint64_t (&strides)[3], const uint32_t (&box)[4]) {
   std::call_once(g_once, load_entry_points);
   if (!g_tiled) {
     set_error("cuTensorMapEncodeTiled unavailable from the driver");
@@ -126,8 +126,8 @@ int encode_tiled_4d_sw128(CUtensorMap* map, const void* base, int element_bytes,
   // the copy moves bits: 16-bit types need no distinction
   CUresult r = g_tiled(map, element_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4,
                        const_cast<void*>(base), d, st, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                       element_bytes == 2 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled (4-D) failed (%d)", (int)r);
     return SPINN_CUDA_ECUDA;
