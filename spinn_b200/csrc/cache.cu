@@ -99,70 +99,84 @@ struct AppendParams {
   int tokens;
 };
 
-// One warp copies one token's key rows or value rows (every head): U is the copied unit, a
-// 16-byte vector where pointers, strides and head_dim allow it, one element otherwise.  Bound by
-// launch latency for a decoding step and by HBM for prompts; four independent loads per lane are
-// in flight.
+constexpr int kAppendTokens = 32;  // most tokens of one CTA
+
+// A CTA copies `per` tokens' key and value rows (every head): its first threads find a token's
+// sequence and slot each, then all threads copy, four independent units in flight per thread.
+// U is the copied unit, a 16-byte vector where pointers, strides and head_dim allow it, one
+// element otherwise.  Few tokens get a CTA each (bound by latency); prompts 32 to a CTA, bound by
+// HBM: the chain of lookups (sequence, length, page) is walked once for 128 KB, where a warp to
+// a token walked it for every 2 KB and reached 5.2 TB/s.
 template <typename U, int ESZ>
-__global__ void __launch_bounds__(256) append_kernel(const AppendParams p) {
-  const int lane = threadIdx.x & 31;
-  const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int tok = (int)(unit >> 1);
-  const bool is_v = unit & 1;
-  if (tok >= p.tokens) return;
-  int seq = tok, first = tok;
-  if (p.starts) {
-    // the last sequence whose first row is at or before tok (empty sequences share their start)
-    int lo = 0, hi = p.c.seqs;  // starts[lo] <= tok < starts[hi]
-    if (p.starts[0] > tok || p.starts[hi] <= tok) {
-      if (lane == 0) atomicOr(p.c.err, kCacheBadLength);
-      return;
+__global__ void __launch_bounds__(256) append_kernel(const AppendParams p, int per) {
+  __shared__ long long slots[kAppendTokens];
+  const int t0 = blockIdx.x * per, tokens = min(per, p.tokens - t0);
+  griddep_launch_dependents();
+  griddep_wait();
+  if ((int)threadIdx.x < tokens) {
+    const int tok = t0 + threadIdx.x;
+    long long slot = -1;
+    unsigned err = 0;
+    int seq = tok, first = tok;
+    if (p.starts) {
+      // the last sequence whose first row is at or before tok (empty sequences share their start)
+      int lo = 0, hi = p.c.seqs;  // starts[lo] <= tok < starts[hi]
+      if (p.starts[0] > tok || p.starts[hi] <= tok) err = kCacheBadLength;
+      while (!err && hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (p.starts[mid] <= tok)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      seq = lo;
+      first = p.starts[lo];
     }
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (p.starts[mid] <= tok)
-        lo = mid;
-      else
-        hi = mid;
+    if (!err) {
+      const int past = p.c.lens[seq];
+      const long long pos = (long long)past + (tok - first);
+      if (past < 0 || tok < first || pos >= cache_capacity(p.c.max_pages, p.c.page_size)) {
+        err = kCacheBadLength;
+      } else {
+        slot = cache_slot(p.c.table + seq * p.c.table_stride, (int)pos, p.c.page_size, p.c.num_pages, p.c.page_stride,
+                          p.c.token_stride);
+        if (slot < 0) err = kCacheBadPage;
+      }
     }
-    seq = lo;
-    first = p.starts[lo];
+    if (err) atomicOr(p.c.err, err);
+    slots[threadIdx.x] = slot;
   }
-  const long long pos = (long long)p.c.lens[seq] + (tok - first);
-  if (p.c.lens[seq] < 0 || pos >= cache_capacity(p.c.max_pages, p.c.page_size)) {
-    if (lane == 0) atomicOr(p.c.err, kCacheBadLength);
-    return;
-  }
-  const long long slot = cache_slot(p.c.table + seq * p.c.table_stride, (int)pos, p.c.page_size, p.c.num_pages,
-                                    p.c.page_stride, p.c.token_stride);
-  if (slot < 0) {
-    if (lane == 0) atomicOr(p.c.err, kCacheBadPage);
-    return;
-  }
-  constexpr int PER = sizeof(U) / ESZ;
-  const int row = p.c.dim / PER, total = row * p.c.kv_heads;
-  const long long src_tok = is_v ? p.v_tok : p.k_tok, src_head = is_v ? p.v_head : p.k_head;
-  const U* src = reinterpret_cast<const U*>(static_cast<const char*>(is_v ? p.v : p.k) + tok * src_tok * ESZ);
-  U* dst = reinterpret_cast<U*>(static_cast<char*>(is_v ? p.c.v : p.c.k) + slot * ESZ);
-  const long long sh = src_head / PER, dh = p.c.head_stride / PER;
-  for (int i0 = lane; i0 < total; i0 += 128) {
-    U r[4];
+  __syncthreads();
+  constexpr int PER = sizeof(U) / ESZ, Q = 4;
+  const int row = p.c.dim / PER, width = row * p.c.kv_heads, total = tokens * width;
+  const U* ks = static_cast<const U*>(p.k) + t0 * (p.k_tok / PER);
+  const U* vs = static_cast<const U*>(p.v) + t0 * (p.v_tok / PER);
+  U* kd = static_cast<U*>(p.c.k);
+  U* vd = static_cast<U*>(p.c.v);
+  const long long kt = p.k_tok / PER, kh = p.k_head / PER, vt = p.v_tok / PER, vh = p.v_head / PER;
+  const long long dh = p.c.head_stride / PER;
+  for (int i0 = threadIdx.x; i0 < total; i0 += Q * 256) {
+    U a[Q], b[Q];
+    long long to[Q];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = i0 + 32 * j;
+    for (int q = 0; q < Q; ++q) {
+      const int i = i0 + q * 256;
+      to[q] = -1;
       if (i < total) {
-        const int h = i / row;
-        r[j] = src[h * sh + (i - h * row)];
+        const int t = i / width, e = i - t * width, h = e / row, c = e - h * row;
+        if (slots[t] >= 0) {
+          to[q] = slots[t] / PER + h * dh + c;
+          a[q] = ks[t * kt + h * kh + c];
+          b[q] = vs[t * vt + h * vh + c];
+        }
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = i0 + 32 * j;
-      if (i < total) {
-        const int h = i / row;
-        dst[h * dh + (i - h * row)] = r[j];
+    for (int q = 0; q < Q; ++q)
+      if (to[q] >= 0) {
+        kd[to[q]] = a[q];
+        vd[to[q]] = b[q];
       }
-    }
   }
 }
 
@@ -792,18 +806,14 @@ __attribute__((visibility("default"))) int spinn_cuda_cache_append(const SpinnCu
   const int per = 16 / es;
   const bool vec = cache_vec16(p.c, es) && aligned16(p.k) && aligned16(p.v) && p.k_tok % per == 0 &&
                    p.k_head % per == 0 && p.v_tok % per == 0 && p.v_head % per == 0;
-  const unsigned blocks = (unsigned)((2ll * p.tokens + 7) / 8);
+  // two CTAs or more to an SM before a CTA takes more tokens
+  const int each = std::max(1, std::min(kAppendTokens, p.tokens / (4 * sm_count(dev))));
+  const dim3 grid((unsigned)((p.tokens + each - 1) / each));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (vec && es == 2)
-    append_kernel<uint4, 2><<<blocks, 256, 0, st>>>(p);
-  else if (vec)
-    append_kernel<uint4, 4><<<blocks, 256, 0, st>>>(p);
-  else if (es == 2)
-    append_kernel<uint16_t, 2><<<blocks, 256, 0, st>>>(p);
-  else
-    append_kernel<uint32_t, 4><<<blocks, 256, 0, st>>>(p);
-  SPINN_CUDA_TRY(cudaGetLastError());
-  return 0;
+  if (vec && es == 2) return launch_dependent(append_kernel<uint4, 2>, grid, 256, 0, st, p, each);
+  if (vec) return launch_dependent(append_kernel<uint4, 4>, grid, 256, 0, st, p, each);
+  if (es == 2) return launch_dependent(append_kernel<uint16_t, 2>, grid, 256, 0, st, p, each);
+  return launch_dependent(append_kernel<uint32_t, 4>, grid, 256, 0, st, p, each);
 }
 
 __attribute__((visibility("default"))) int spinn_cuda_cache_evict(const SpinnCudaCache* cache,

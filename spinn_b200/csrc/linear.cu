@@ -560,6 +560,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 res[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.res) +
                                                               (long long)(m0 + c + orow + 2 * j) * p.ldr + on));
           }
+          // the same for rows off alignment, as they are stored below
+          const int n0 = (tn * PAIR + (PAIR == 2 ? rank : 0)) * 128, width = min(128, p.n - n0);
+          T loose[4][3][2];
+          if (p.res && !p.vec_y) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int row = quarter * 4 + q;
+              const T* extra = static_cast<const T*>(p.res) + (long long)(m0 + c + row) * p.ldr + n0;
+              const int odd = ((uintptr_t)(static_cast<T*>(p.y) + (long long)(m0 + c + row) * p.ldy + n0) >> 1) & 1;
+#pragma unroll
+              for (int j = 0; j < 3; ++j) {
+                const int e = 2 * (lane + 32 * j) - odd;
+                const bool live = row < rows && !(j == 2 && e > 127);
+                if (live && e >= 0 && e < width) loose[q][j][0] = extra[e];
+                if (live && e + 1 >= 0 && e + 1 < width) loose[q][j][1] = extra[e + 1];
+              }
+            }
+          }
           tmem_ld_wait();
           float v[CW];
 #pragma unroll
@@ -598,12 +616,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
           } else {
             // rows off alignment: 4-byte words at the row's own parity, its ends in single elements
-            const int n0 = (tn * PAIR + (PAIR == 2 ? rank : 0)) * 128, width = min(128, p.n - n0);
             for (int q = 0; q < 4; ++q) {
               const int row = quarter * 4 + q;
               if (row >= rows) break;
               T* dst = static_cast<T*>(p.y) + (long long)(m0 + c + row) * p.ldy + n0;
-              const T* extra = p.res ? static_cast<const T*>(p.res) + (long long)(m0 + c + row) * p.ldr + n0 : nullptr;
               const float* src = stage + row * C::STG_PITCH;
               const int odd = ((uintptr_t)dst >> 1) & 1;
 #pragma unroll
@@ -611,14 +627,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 const int e = 2 * (lane + 32 * j) - odd;
                 if (e >= width || (j == 2 && e > 127)) continue;
                 const bool first = e >= 0, second = e + 1 < width;
-                float o0 = first ? src[e] : 0.0f, o1 = second ? src[e + 1] : 0.0f;
-                if (extra) {
-                  if (first) o0 += to_float(extra[e]);
-                  if (second) o1 += to_float(extra[e + 1]);
-                }
+                const float o0 = first ? src[e] : 0.0f, o1 = second ? src[e + 1] : 0.0f;
                 Pair<T> x;
-                x.t[0] = round_to<T>(o0);
-                x.t[1] = round_to<T>(o1);
+                x.t[0] = round_to<T>(p.res ? o0 + to_float(loose[q][j][0]) : o0);
+                x.t[1] = round_to<T>(p.res ? o1 + to_float(loose[q][j][1]) : o1);
                 if (first && second)
                   *reinterpret_cast<uint32_t*>(dst + e) = x.u;
                 else if (first)
