@@ -34,7 +34,11 @@ class Paged:
                 return flat[1:].view(total, page, kv_heads, dim + 1)[..., :dim]
             return torch.full((total, page, kv_heads, dim), float("nan"), dtype=dt)
 
-        k, v = pool(), pool()
+        if layout == "pair":         # keys and values of a page side by side in one tensor
+            both = torch.full((total, 2, page, kv_heads, dim), float("nan"), dtype=dt)
+            k, v = both[:, 0], both[:, 1]
+        else:
+            k, v = pool(), pool()
         for s, n in enumerate(lens):
             t = np.arange(n)
             p, o = torch.from_numpy(table[s, t // page].astype(np.int64)), torch.from_numpy(t % page)
@@ -46,7 +50,11 @@ class Paged:
             base = t._base if t._base is not None else t
             return base.to(device).as_strided(t.shape, t.stride(), t.storage_offset())
 
-        self.k, self.v = put(k), put(v)
+        if layout == "pair":
+            both = put(both)
+            self.k, self.v = both[:, 0], both[:, 1]
+        else:
+            self.k, self.v = put(k), put(v)
         self.table = torch.from_numpy(table).to(device)
         self.lens = torch.tensor(list(lens), dtype=torch.int32, device=device)
 

@@ -79,6 +79,10 @@ ATTENTIONS = [
     ("fp32", [50, 81], 3, 1, 7, 3, "odd", True),
     ("fp16", [4097], 8, 8, 128, 64, "nhd", True),               # one long sequence in many shares
     ("bf16", [5000], 1, 1, 64, 16, "nhd", True),
+    ("fp16", [512, 511, 1], 8, 2, 64, 16, "pair", True),        # the longest tables that are not split
+    ("bf16", [513, 512, 0, 700], 8, 4, 128, 32, "pair", True),  # and the shortest that are
+    ("fp32", [256, 7], 4, 2, 64, 8, "pair", True),
+    ("fp32", [257, 300], 2, 2, 128, 16, "pair", False),
 ]
 
 
@@ -148,6 +152,151 @@ def test_attention_scores_far_apart(rt):
     want, _, absum, ds = decode_ref.attention(c, q, 1.0)
     tol = 2.0 ** -11 * want.abs() + 2 * (ds + 2.0 ** -16) * absum + 150 * 2.0 ** -25 * 6
     assert ((y.cpu().double() - want).abs() <= tol).all()
+
+
+def _check_on_gpu(c, q, y, win, wout, dtype):
+    """As _check_attention, for many sequences: 64 bits on the GPU, one sequence at a time."""
+    half, dim = torch.finfo(DTYPES[dtype]).eps / 2, q.shape[2]
+    group = q.shape[1] // c.heads
+    for s, n in enumerate(c.lens_host):
+        if n == 0:
+            assert bool((y[s] == 0).all())
+            continue
+        t = torch.arange(n, device="cuda")
+        pages = c.table[s].long()[t // c.page]
+        k = c.k[pages, t % c.page].double().repeat_interleave(group, 1).transpose(0, 1)   # [heads, n, dim]
+        v = c.v[pages, t % c.page].double().repeat_interleave(group, 1).transpose(0, 1)
+        qs = q[s].double()
+        p = torch.softmax(torch.einsum("hd,hnd->hn", qs, k) * dim ** -0.5, -1)
+        want, absum = torch.einsum("hn,hnd->hd", p, v), torch.einsum("hn,hnd->hd", p, v.abs())
+        ds = torch.einsum("hd,hnd->hn", qs.abs(), k.abs()).amax(-1, keepdim=True) * dim ** -0.5 * dim * 2.0 ** -24
+        rel = 2 * (ds + 2.0 ** -21 + n * 2.0 ** -24) + (2.0 ** -17 if dtype != "fp32" else 0.0)
+        tiny = n * 2.0 ** -25 * 6 if dtype == "fp16" else 0.0
+        assert ((y[s].double() - want).abs() <= half * want.abs() + rel * absum * (1 + half) + tiny).all(), s
+        if wout is not None:
+            mass = p.view(c.heads, group, n).sum(1)
+            ref = win[s, :, :n].double() + mass
+            r = rel.view(c.heads, group, 1).amax(1)
+            assert ((wout[s, :, :n].double() - ref).abs() <= r * mass + ref.abs() * 2.0 ** -23).all(), s
+
+
+@pytest.mark.parametrize("dtype,seqs,most,q_heads,heads,dim,page,layout", [
+    ("bf16", 300, 700, 16, 4, 64, 16, "nhd"),     # more sequences than threads: scanned in parts
+    ("fp16", 129, 90, 8, 8, 128, 24, "nhd"),      # lanes copying, many short ones to a share
+    ("bf16", 64, 2300, 16, 8, 64, 32, "hnd"),     # shares of more than 32 tiles
+    ("fp32", 200, 400, 6, 3, 80, 8, "nhd"),
+    ("fp16", 40, 3000, 14, 2, 128, 7, "nhd"),     # a group of seven, pages that end inside every tile
+])
+def test_attention_over_large_batches(rt, dtype, seqs, most, q_heads, heads, dim, page, layout):
+    rng = np.random.default_rng(seqs)
+    lens = [int(x) for x in rng.integers(0, most + 1, seqs)]
+    lens[3], lens[7], lens[-1] = 0, most, 0
+    c = Paged(dtype, lens, heads, dim, page, seed=seqs, layout=layout)
+    q = (torch.randn(seqs, q_heads, dim, device="cuda") * 2).to(DTYPES[dtype])
+    y = torch.full_like(q, float("nan"))
+    win = torch.rand(seqs, heads, most, device="cuda")
+    wout = torch.full((seqs, heads, most), -3.0, device="cuda")
+    rt.paged_attention(q, c.k, c.v, c.table, c.lens, y, None, win, wout)
+    rt.stream_sync()
+    _check_on_gpu(c, q, y, win, wout, dtype)
+    y2 = torch.full_like(q, float("nan"))
+    rt.paged_attention(q, c.k, c.v, c.table, c.lens, y2)
+    rt.stream_sync()
+    assert torch.equal(y, y2)
+    late = torch.arange(most, device="cuda") >= c.lens[:, None]
+    assert bool((wout.transpose(1, 2)[late] == -3.0).all())
+
+
+def test_calls_at_once_on_two_streams(rt):
+    """Eager calls that overlap on the GPU, each on its own stream with its own workspace."""
+    runs = []
+    for i in range(2):
+        c, q, y, win, wout = _attention_case(rt, ("bf16", [4000, 300, 0, 2500], 16, 4, 128, 16, "nhd", True), seed=40 + i)
+        runs.append((c, q, y, win, wout, torch.cuda.Stream()))
+    x = [torch.randn(200, 1001, device="cuda").half() for _ in range(2)]      # with aligned copies
+    w = torch.randn(600, 1001, device="cuda").half()
+    want = [torch.empty(200, 600, device="cuda").half() for _ in range(2)]
+    for a, b in zip(x, want):
+        rt.linear(a, w, b)
+    rt.stream_sync()
+    for _ in range(10):
+        outs = []
+        for i, (c, q, y, win, wout, stream) in enumerate(runs):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                z, y2, w2 = torch.empty_like(want[i]), torch.zeros_like(y), torch.full_like(wout, -3.0)
+                rt.paged_attention(q, c.k, c.v, c.table, c.lens, y2, None, win, w2)
+                rt.linear(x[i], w, z)
+                outs.append((y2, w2, z))
+        torch.cuda.synchronize()
+        for (c, q, y, win, wout, _s), b, (y2, w2, z) in zip(runs, want, outs):
+            assert torch.equal(y, y2) and torch.equal(wout, w2) and torch.equal(b, z)
+
+
+def test_captured_between_other_nodes(rt):
+    """A graph whose calls follow copies, memsets, torch kernels and a join of two streams."""
+    c, q, y, win, wout = _attention_case(rt, ("bf16", [700, 33], 8, 2, 64, 16, "nhd", True))
+    new = torch.randn(2, 2, 64, device="cuda").to(torch.bfloat16)
+    q0, w0 = q.clone(), win.clone()
+    y2, w2, src = torch.empty_like(y), torch.zeros_like(wout), torch.zeros_like(q)
+    scratch = torch.empty(1 << 20, device="cuda")
+    graph, main, side = torch.cuda.CUDAGraph(), torch.cuda.Stream(), torch.cuda.Stream()
+    mat, out = torch.randn(64, 64, device="cuda").to(torch.bfloat16), torch.empty(16, 64, device="cuda").to(torch.bfloat16)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=main):
+        src.copy_(q0)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            scratch.zero_()
+            rt.linear(q0.view(16, 64), mat, out)
+        w2.fill_(-3.0)
+        main.wait_stream(side)
+        rt.paged_attention(src, c.k, c.v, c.table, c.lens, y2, None, w0, w2)
+        scratch.add_(1.0)
+    for _ in range(3):
+        y2.zero_()
+        graph.replay()
+        rt.stream_sync()
+        assert torch.equal(y2, y) and torch.equal(w2[:, :, :700], wout[:, :, :700])
+    del new
+
+
+FIRST_CALLS = """
+import torch
+from spinn_b200 import runtime as rt
+dt = torch.bfloat16
+k = torch.randn(40, 16, 2, 64, device="cuda").to(dt); v = k.clone()
+table = torch.arange(40, dtype=torch.int32, device="cuda").view(2, 20); lens = torch.tensor([100, 7], dtype=torch.int32, device="cuda")
+q = torch.randn(2, 8, 64, device="cuda").to(dt); y = torch.empty_like(q)
+w = torch.zeros(2, 2, 320, device="cuda"); new = torch.empty(2, dtype=torch.int32, device="cuda")
+kept = torch.empty(2, 2, 50, dtype=torch.int32, device="cuda")
+row = torch.randn(2, 2, 64, device="cuda").to(dt)
+x = torch.randn(40, 65, device="cuda").to(dt); m = torch.randn(32, 65, device="cuda").to(dt); z = torch.empty(40, 32, device="cuda").to(dt)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    rt.cache_append(row, row, k, v, table, lens)
+    rt.paged_attention(q, k, v, table, lens, y, None, w, w)
+    rt.linear(x, m, z)
+    rt.linear(x[:3], m, z[:3])
+    rt.cache_evict(k, v, table, lens, w, w, table, new, kept, 50)
+g.replay()
+rt.stream_sync()
+assert new.tolist() == [50, 7] and abs(float(w[1].sum()) - 8) < 1e-4 and torch.isfinite(z.float()).all()
+print("replayed")
+"""
+
+
+def test_first_calls_of_a_process_may_be_captured(cuda_lib):
+    """Nothing is allocated or asked of the device that a capture forbids, not even the first time."""
+    import os
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+    r = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=ROOT, capture_output=True, text=True, timeout=300,
+                       env=dict(os.environ, PYTHONPATH=ROOT))
+    assert r.returncode == 0 and "replayed" in r.stdout, r.stderr[-2000:]
 
 
 def test_attention_is_deterministic_and_replays(rt):

@@ -144,3 +144,42 @@ def test_linear_captured_and_replayed(rt):
     graph.replay()
     rt.stream_sync()
     assert torch.equal(y, y2)
+
+
+def test_linear_rows_far_apart(rt):
+    """Row strides that carry past 2^31 elements, in y, the residual and x."""
+    far = (1 << 30) + 8
+    big = torch.zeros(2 * far + 4096, dtype=torch.bfloat16, device="cuda")
+    for m in (3, 20):
+        step = 2 * far // (m - 1) // 8 * 8
+        view = big.as_strided((m, 64), (step, 1))
+        x = rows((m, 72), torch.bfloat16)
+        w = rows((64, 72), torch.bfloat16, scale=0.1)
+        y = torch.empty(m, 64, dtype=torch.bfloat16, device="cuda")
+        view.copy_(torch.randn(m, 64, device="cuda"))
+        res = view.clone()
+        rt.linear(x, w, y, None, res)
+        rt.linear(x, w, view, None, view)
+        rt.stream_sync()
+        assert torch.equal(view, y)
+        z = torch.empty(m, 16, dtype=torch.bfloat16, device="cuda")
+        rt.linear(view, w[:16, :64], z)                 # x with far rows; w off alignment
+        want = y.double() @ w[:16, :64].double().T
+        mass = y.double().abs() @ w[:16, :64].double().abs().T
+        rt.stream_sync()
+        assert ((z.double() - want).abs() <= 2.0 ** -8 * want.abs() + 64 * 2.0 ** -23 * mass).all()
+
+
+@pytest.mark.parametrize("m", [1, 8, 9, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257])
+def test_linear_around_the_tile_sizes(rt, m):
+    for k, n in ((128, 128), (136, 256), (1032, 264), (4104, 40), (8, 1032)):
+        torch.manual_seed(m + k + n)
+        x, w = rows((m, k), torch.float16), rows((n, k), torch.float16, scale=k ** -0.5)
+        y, r, b = rows((m, n), torch.float16), rows((m, n), torch.float16), torch.randn(n, device="cuda").half()
+        rt.linear(x, w, y, b, r, "silu")
+        rt.stream_sync()
+        z = x.double() @ w.double().T + b.double()
+        mass = x.double().abs() @ w.double().abs().T
+        want = act64(z, "silu") + r.double()
+        slack = 1.13 * k * 2.0 ** -23 * mass + 2.0 ** -20 * (z.abs() + 1) + 2.0 ** -22 * (z.abs() + want.abs())
+        assert ((y.double() - want).abs() <= 2.0 ** -11 * want.abs() + 1.001 * slack + 2.0 ** -25).all(), (m, k, n)
