@@ -358,7 +358,6 @@ struct LinCfg {
   static constexpr int SMEM = STAGES * STAGE + PART + STG + 512 + 1024;
   static_assert(COLS <= 512, "TMEM");
   static_assert(STAGES >= 2, "pipeline needs two stages");
-  static_assert(!SPL || PAIR == 1, "a cluster is either a pair or a split");
 };
 
 template <typename T, typename C>
@@ -381,9 +380,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = PAIR == 2 || SPL ? cluster_ctarank() : 0;
-  const uint32_t splits = SPL ? cluster_size() : 1;
-  const int unit0 = SPL ? blockIdx.x / splits : blockIdx.x / PAIR;
+  const uint32_t crank = PAIR == 2 || SPL ? cluster_ctarank() : 0;
+  const uint32_t side = PAIR == 2 ? crank & 1 : 0, leader = crank - side;  // place in the pair, its leader
+  const uint32_t rank = SPL ? crank / PAIR : 0;                              // place in the split
+  const uint32_t splits = SPL ? cluster_size() / PAIR : 1;
+  const int unit0 = SPL ? blockIdx.x / (splits * PAIR) : blockIdx.x / PAIR;
   const int step = SPL ? p.num_tiles : gridDim.x / PAIR;  // a cluster has one tile
   const int kb0 = SPL ? (int)((long long)p.num_kb * rank / splits) : 0;
   const int kb1 = SPL ? (int)((long long)p.num_kb * (rank + 1) / splits) : p.num_kb;
@@ -417,7 +418,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   tc_fence_before();
   __syncthreads();
   if constexpr (PAIR == 2) cluster_sync();  // the peer's barriers are initialised before use
-  if constexpr (SPL) cluster_arrive();      // waited for before the first store to another CTA
+  if constexpr (SPL && PAIR == 1) cluster_arrive();  // waited for before the first store to another CTA
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   griddep_launch_dependents();
@@ -439,12 +440,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     for (int t = unit0; t < p.num_tiles && !warp_abort(abort_flag); t += step) {
       int tm, tn;
       decode(t, &tm, &tn);
-      const int w_row = (tn * PAIR + (PAIR == 2 ? rank : 0)) * 128;
-      const int x_row = tm * BN + (PAIR == 2 ? rank * (BN / 2) : 0);
+      const int w_row = (tn * PAIR + side) * 128;
+      const int x_row = tm * BN + side * (BN / 2);
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!warp_wait_bar(&empty[s], ph ^ 1, abort_flag)) break;
         if (lane == 0) {
-          if (PAIR == 1 || rank == 0) {
+          if (side == 0) {
             mbar_arrive_expect_tx(&full[s], C::STAGE * PAIR);
             armed |= 1u << s;
             armed_ph = (armed_ph & ~(1u << s)) | (ph << s);
@@ -454,7 +455,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             uint8_t *a = sA + s * C::A_STAGE + h * C::A_SPAN, *b = sB + s * C::B_STAGE + h * C::B_SPAN;
             const int k = kb * C::BK + h * C::SPAN;
             if constexpr (PAIR == 2) {
-              const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+              const uint32_t bar = mapa_shared(smem_u32(&full[s]), leader);
               tma_load_2d_pair(&mapW, bar, a, k, w_row);
               tma_load_2d_pair(&mapX, bar, b, k, x_row);
             } else {
@@ -477,7 +478,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (armed & (1u << i)) mbar_wait(&full[i], (armed_ph >> i) & 1, &dummy, kDrainNs);
     }
     __syncwarp();
-  } else if (warp == 1 && (PAIR == 1 || rank == 0)) {
+  } else if (warp == 1 && side == 0) {
     // ---- MMA issuer (the pair's leader)
     constexpr uint32_t idesc = make_idesc_16<T>(128 * PAIR, BN);
     const uint64_t adesc = make_smem_desc(smem_u32(sA), 16, 1024, kSw128);
@@ -509,8 +510,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               umma_f16(tmem + b * BN, aj, xj, idesc, acc);
           }
           if constexpr (PAIR == 2) {
-            umma_commit_pair(mapa_shared(smem_u32(&empty[s]), 0));
-            umma_commit_pair(mapa_shared(smem_u32(&empty[s]), 1));
+            umma_commit_pair(mapa_shared(smem_u32(&empty[s]), leader));
+            umma_commit_pair(mapa_shared(smem_u32(&empty[s]), leader + 1));
           } else {
             umma_commit(&empty[s]);
           }
@@ -525,8 +526,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (!ok) break;
       if (lane == 0) {
         if constexpr (PAIR == 2) {
-          umma_commit_pair(mapa_shared(smem_u32(&tfull[b]), 0));
-          umma_commit_pair(mapa_shared(smem_u32(&tfull[b]), 1));
+          umma_commit_pair(mapa_shared(smem_u32(&tfull[b]), leader));
+          umma_commit_pair(mapa_shared(smem_u32(&tfull[b]), leader + 1));
         } else {
           umma_commit(&tfull[b]);
         }
@@ -536,7 +537,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (warp_abort(abort_flag) && issued && lane == 0) {
       volatile int dummy = 0;
       if constexpr (PAIR == 2)
-        umma_commit_pair(mapa_shared(smem_u32(drain), 0));
+        umma_commit_pair(mapa_shared(smem_u32(drain), leader));
       else
         umma_commit(drain);
       mbar_wait(drain, 0, &dummy, kDrainNs);
@@ -546,16 +547,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     // ---- epilogue: warp pairs share a TMEM lane quarter and alternate over its column chunks
     constexpr int CW = 16;  // columns (rows of x) per step
     const int quarter = warp & 3, half = (warp - 4) >> 2;
-    if constexpr (SPL) cluster_wait();  // the cluster's other CTAs run: their shared memory may be written
+    if constexpr (SPL && PAIR == 1) cluster_wait();  // the cluster's other CTAs run: they may be written to
     int it = 0;
     for (int t = unit0; t < p.num_tiles; t += step, ++it) {
       int tm, tn;
       decode(t, &tm, &tn);
-      const int n = (tn * PAIR + (PAIR == 2 ? rank : 0)) * 128 + quarter * 32 + lane;
+      const int n = (tn * PAIR + side) * 128 + quarter * 32 + lane;
       const int m0 = tm * BN;
       const float bias = !SPL && p.bias && n < p.n ? to_float(static_cast<const T*>(p.bias)[n]) : 0.0f;
       const int b = it % NACC;
-      if (!__all_sync(0xffffffffu, mbar_wait_backoff(&tfull[b], (it / NACC) & 1, abort_flag, kTimeoutNs))) break;
+      const bool ok = __all_sync(0xffffffffu, mbar_wait_backoff(&tfull[b], (it / NACC) & 1, abort_flag, kTimeoutNs));
+      if (!ok) break;
       tc_fence_after();
       for (int c = half * CW; c < BN && m0 + c < p.m; c += 2 * CW) {
         uint32_t r[CW];
@@ -568,11 +570,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
           for (int i = 0; i < CW; i += 4) {
             const uint32_t g = (c + i) >> 2, to = g & (splits - 1), slot = g / splits;
-            if (i < rows) st_cluster_v4(mapa_shared(mine + slot * 2048, to), r[i], r[i + 1], r[i + 2], r[i + 3]);
+            if (i < rows) st_cluster_v4(mapa_shared(mine + slot * 2048, to * PAIR + side), r[i], r[i + 1], r[i + 2], r[i + 3]);
           }
         } else {
           // this thread's part of the output: eight consecutive n of two rows of x
-          const int on = (tn * PAIR + (PAIR == 2 ? rank : 0)) * 128 + (lane & 15) * 8;
+          const int on = (tn * PAIR + side) * 128 + (lane & 15) * 8;
           const int orow = quarter * 4 + (lane >> 4);
           uint4 res[2];
           if (p.res && p.vec_y && on + 8 <= p.n) {
@@ -583,7 +585,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                                               (long long)(m0 + c + orow + 2 * j) * p.ldr + on));
           }
           // the same for rows off alignment, as they are stored below
-          const int n0 = (tn * PAIR + (PAIR == 2 ? rank : 0)) * 128, width = min(128, p.n - n0);
+          const int n0 = (tn * PAIR + side) * 128, width = min(128, p.n - n0);
           T loose[4][3][2];
           if (p.res && !p.vec_y) {
 #pragma unroll
@@ -668,7 +670,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       __syncwarp();
       if (lane == 0) {
         if constexpr (PAIR == 2)
-          mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[b]), 0));
+          mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[b]), leader));
         else
           mbar_arrive(&tempty[b]);
       }
@@ -683,7 +685,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     decode(unit0, &tm, &tn);
     const int rows = min(BN, p.m - tm * BN), groups = (rows + 3) >> 2;
     const int mine = (groups - (int)rank + (int)splits - 1) / (int)splits;  // groups rank, rank + splits, ...
-    const int n = tn * 128 + 2 * (threadIdx.x & 63);
+    const int n = (tn * PAIR + side) * 128 + 2 * (threadIdx.x & 63);
     const bool one = n < p.n, two = n + 1 < p.n;
     const float bias0 = p.bias && one ? to_float(static_cast<const T*>(p.bias)[n]) : 0.0f;
     const float bias1 = p.bias && two ? to_float(static_cast<const T*>(p.bias)[n + 1]) : 0.0f;
@@ -702,7 +704,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         res[e][1] = live && two ? to_float(src[1]) : 0.0f;
       }
       if (!joined) {
-        if (warp < 4) cluster_wait();
+        if (PAIR == 1 && warp < 4) cluster_wait();
         cluster_arrive();
         cluster_wait();
         joined = true;
@@ -774,7 +776,8 @@ LinearPlan linear_plan(const LinearParams& p, int sms) {
   // Shape by estimated clocks, fitted to a sweep of every shape over 30 sizes (device time in a
   // captured queue).  A stage of 128 k takes as long as its operands need to pass through shared
   // memory twice (written by TMA, read by the MMA at 128 bytes a clock): about 870 clocks for a
-  // single CTA whatever its width up to 128, 950 and 1,150 for the pairs.  Around the stages lie
+  // single CTA whatever its width up to 128, 950 and 1,150 for the pairs (700 for split ones, which run
+  // alone on memory-bound problems).  Around the stages lie
   // the launch and first loads (2,600; 900 more for a cluster), and the last tile's epilogue.
   // Splitting k pays when there are few tiles: it adds the exchange of the partial sums.
   const int kb = (p.k + 127) / 128;
@@ -783,10 +786,12 @@ LinearPlan linear_plan(const LinearParams& p, int sms) {
     const long long tiles = (long long)((p.m + bn - 1) / bn) * ((p.n + 128 * pair - 1) / (128 * pair));
     const long long waves = (tiles * pair * split + sms - 1) / sms;
     if (split > 1 && (waves > 1 || kb < 2 * split)) return;
-    const double stage = pair == 1 ? 870.0 : bn == 256 ? 1150.0 : 950.0;
+    // clusters that the GPCs of 148 SMs hold at once
+    if (split > 1 && (split * pair == 8 ? tiles > 15 : split * pair == 4 && tiles > 34)) return;
+    const double stage = pair == 1 ? 870.0 : bn == 256 ? 1150.0 : split > 1 ? 700.0 : 950.0;
     double clocks = 2600.0 + (pair * split > 1 ? 900.0 : 0.0) + (double)waves * ((kb + split - 1) / split) * stage;
     clocks += bn * 30.0 + 300.0;
-    if (split > 1) clocks += 1100.0 + bn * 26.0 / split;
+    if (split > 1) clocks += 1100.0 + bn * 26.0 / split + (pair == 2 ? 1700.0 : 0.0);
     if (pl.bn == 0 || clocks < best) {
       pl.bn = bn;
       pl.pair = pair;
@@ -796,7 +801,7 @@ LinearPlan linear_plan(const LinearParams& p, int sms) {
   };
   for (int split = 1; split <= 8; split *= 2)
     for (int bn = 32; bn <= 128; bn *= 2) consider(bn, 1, split);
-  consider(128, 2, 1);
+  for (int split = 1; split <= 4; split *= 2) consider(128, 2, split);
   consider(256, 2, 1);
   return pl;
 }
@@ -819,8 +824,8 @@ int launch_tiles(const LinearParams& p0, const LinearPlan& pl, const void* x, lo
   if (rc) return rc;
   auto* kernel = linear_tile_kernel<T, C>;
   SPINN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-  const int cluster = C::SPL ? pl.split : C::PAIR;
-  const int grid = C::SPL ? p.num_tiles * pl.split : std::min(p.num_tiles, sms / C::PAIR) * C::PAIR;
+  const int cluster = C::SPL ? pl.split * C::PAIR : C::PAIR;
+  const int grid = C::SPL ? p.num_tiles * cluster : std::min(p.num_tiles, sms / C::PAIR) * C::PAIR;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(kTileThreads);
@@ -875,10 +880,11 @@ int linear_launch(const LinearParams& p, const LinearPlan& pl, void* ws, int sms
     const int rc = launch_dependent(pitch_kernel, dim3((unsigned)std::min((std::max(c.rows[0], c.rows[1]) + 7) / 8, sms * 8), 2), 256, 0, st, c);
     if (rc) return rc;
   }
-  if (pl.pair == 2)
-    return pl.bn == 256 ? launch_tiles<T, LinCfg<256, 2, false>>(p, pl, x, ldx, w, ldw, sms, st)
-                        : launch_tiles<T, LinCfg<128, 2, false>>(p, pl, x, ldx, w, ldw, sms, st);
   const bool spl = pl.split > 1;
+  if (pl.pair == 2 && pl.bn == 256) return launch_tiles<T, LinCfg<256, 2, false>>(p, pl, x, ldx, w, ldw, sms, st);
+  if (pl.pair == 2)
+    return spl ? launch_tiles<T, LinCfg<128, 2, true>>(p, pl, x, ldx, w, ldw, sms, st)
+               : launch_tiles<T, LinCfg<128, 2, false>>(p, pl, x, ldx, w, ldw, sms, st);
 #define LINEAR_BN(W)                                                                        \
   if (pl.bn == W)                                                                           \
     return spl ? launch_tiles<T, LinCfg<W, 1, true>>(p, pl, x, ldx, w, ldw, sms, st)        \
