@@ -84,7 +84,7 @@ __attribute__((visibility("default"))) size_t spinn_cuda_paged_attention_workspa
     return 0;
   }
   const AttnPlan pl = attention_plan(p, cache->dtype, sm_count(dev));
-  return pl.part + pl.ml + pl.pieces + pl.logits;
+  return pl.part + pl.ml + pl.pieces + pl.segs + pl.logits;
 }
 
 __attribute__((visibility("default"))) int spinn_cuda_paged_attention(const SpinnCudaCache* cache,
@@ -100,14 +100,15 @@ __attribute__((visibility("default"))) int spinn_cuda_paged_attention(const Spin
   rc = decode_error_word(dev, &p.c.err);
   if (rc) return rc;
   const AttnPlan pl = attention_plan(p, cache->dtype, sm_count(dev));
-  const size_t need = pl.part + pl.ml + pl.pieces + pl.logits;
+  const size_t need = pl.part + pl.ml + pl.pieces + pl.segs + pl.logits;
   SPINN_CHECK_ARG(!need || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                   "paged_attention: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
   char* ws = static_cast<char*>(workspace);
   p.part = reinterpret_cast<float*>(ws);
   p.ml = reinterpret_cast<float*>(ws + pl.part);
   p.pieces = reinterpret_cast<Piece*>(ws + pl.part + pl.ml);
-  p.logits = reinterpret_cast<float*>(ws + pl.part + pl.ml + pl.pieces);
+  p.segs = reinterpret_cast<Segment*>(ws + pl.part + pl.ml + pl.pieces);
+  p.logits = reinterpret_cast<float*>(ws + pl.part + pl.ml + pl.pieces + pl.segs);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return cache->dtype == SPINN_CUDA_FP16   ? attention_launch_fp16(p, pl, st)
          : cache->dtype == SPINN_CUDA_BF16 ? attention_launch_bf16(p, pl, st)

@@ -295,11 +295,14 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
   // empty sequences have no units: their outputs are zeros
   auto clear_empty = [&]() {
     for (int s = me; s < p.c.seqs; s += workers)
-      if (attn_len(p, s) == 0)
+      if (attn_len(p, s) == 0) {
         for (int i = tid; i < p.q_heads * p.c.dim; i += kThreads) {
           const int h = i / p.c.dim;
           static_cast<T*>(p.y)[s * p.y_seq + h * p.y_head + (i - h * p.c.dim)] = from_float<T>(0.0f);
         }
+        if (p.by_segment)
+          for (int i = tid; i < p.hblocks; i += kThreads) p.segs[s * p.hblocks + i] = {0, -1};
+      }
   };
   if (u0 >= u1) {
     if (tid < 2) p.pieces[me * 2 + tid].s = -1;
@@ -821,6 +824,9 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
         r.hi = end <= u1 ? end : u1;
         r.s = cur.s;
       }
+      // its first worker records a split segment for the join, a whole one that there is nothing to
+      if (!p.whole && p.by_segment && tid == 0 && begin >= u0)
+        p.segs[cur.s * p.hblocks + cur.hb] = {me, end > u1 ? AttnShares(units, workers).owner(end - 1) : -1};
     }
     if (i + 1 < count) walk_next<TK>(p, cur);
   }
@@ -832,10 +838,16 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
 }
 
 // ------------------------------------------------------------------ join
-// Block (w, 0): when worker w is the second one of a segment, the block joins the partials of all
-// the segment's workers by an online softmax, four output registers to a warp, the workers dealt
-// to the warps that are left.  Blocks (w, 1 ..), with weights, turn the scores of the worker's own
-// tokens in split segments into probabilities.
+// Joins the partials of split segments by an online softmax, four output registers (a slice) to a
+// warp.  A chain of dependent loads and launches bounds it, so its blocks are laid out for one
+// round of loads:
+//   by_segment (few segments, of many workers each): a block per (segment, slice), the workers
+//     dealt to its sixteen warps, whose states meet in a tree;
+//   else: a block per worker, which joins the segment whose second worker it is, its warps dealt
+//     to the slices first and to the workers with what is left.
+// With weights the first blocks, one per worker, turn the scores of the worker's own tokens in
+// split segments into probabilities.
+// (8 heads of 32768 tokens, 37 workers each: 40.3 us with the second layout alone, XX with both.)
 template <typename T, int DPAD, int GB, bool WTS>
 __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const __grid_constant__ AttnParams p) {
   using C = Tile<T, DPAD, GB>;
@@ -843,15 +855,37 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const _
   constexpr int GROUPS = SLICES >= kJoinWarps ? 1 : kJoinWarps / SLICES;  // warps that share a slice
   griddep_launch_dependents();
   griddep_wait();
-  const int me = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (blockIdx.y == 0) {
-    const Piece pc = p.pieces[me * 2];
-    if (pc.s < 0) return;
-    // the first worker after w0 with a share joins; workers between without one have no piece
-    for (int w = pc.w0 + 1; w < me; ++w)
-      if (p.pieces[w * 2].s >= 0) return;
-    __shared__ float sm[GROUPS > 1 ? kJoinWarps : 1][32][9];
-    for (int slice = warp / GROUPS; slice < SLICES; slice += kJoinWarps / GROUPS) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int weight_blocks = WTS ? p.workers : 0;
+  if ((int)blockIdx.x >= weight_blocks) {
+    const int job = blockIdx.x - weight_blocks;
+    int s, hb, w0, w1, slice, slice_step, group, groups;
+    if (p.by_segment) {
+      const int seg = job / SLICES;
+      const Segment rec = p.segs[seg];
+      if (rec.w1 < 0) return;
+      s = seg / p.hblocks;
+      hb = seg - s * p.hblocks;
+      w0 = rec.w0;
+      w1 = rec.w1;
+      slice = job - seg * SLICES;
+      slice_step = SLICES;
+      group = warp;
+      groups = kJoinWarps;
+    } else {
+      const Piece pc = p.pieces[job * 2];
+      if (pc.s < 0 || pc.w0 + 1 != job) return;
+      s = pc.s;
+      hb = pc.hb;
+      w0 = pc.w0;
+      w1 = pc.w1;
+      slice = warp / GROUPS;
+      slice_step = kJoinWarps / GROUPS;
+      group = warp % GROUPS;
+      groups = GROUPS;
+    }
+    __shared__ float sm[kJoinWarps][32][9];
+    for (; slice < SLICES; slice += slice_step) {
       const int i0 = slice * 4;
       int h0, h1, d[4];
       if constexpr (C::k16) {
@@ -877,14 +911,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const _
         for (int i = 0; i < 4; ++i) o[i] = C::k16 && (i & 1) ? o[i] * f1 + x[i] * e1 : o[i] * f0 + x[i] * e0;
       };
       constexpr int U = 4;  // partials in flight
-      for (int wb = pc.w0 + warp % GROUPS; wb <= pc.w1; wb += U * GROUPS) {
+      for (int wb = w0 + group; wb <= w1; wb += U * groups) {
         float x[U][4], a0[U], a1[U], b0[U], b1[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int w = wb + u * GROUPS, slot = w * 2 + (w == pc.w0 ? 1 : 0);
+          const int w = wb + u * groups, slot = w * 2 + (w == w0 ? 1 : 0);
           a0[u] = a1[u] = kNothing;
           b0[u] = b1[u] = x[u][0] = x[u][1] = x[u][2] = x[u][3] = 0.0f;
-          if (w > pc.w1 || (w != pc.w0 && p.pieces[slot].s < 0)) continue;
+          if (w > w1) continue;
           const float* ml = p.ml + (size_t)slot * 2 * GB;
           const float* src = p.part + ((size_t)slot * NR + i0) * 32 + lane;
 #pragma unroll
@@ -897,36 +931,42 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const _
 #pragma unroll
         for (int u = 0; u < U; ++u) add(a0[u], a1[u], b0[u], b1[u], x[u]);
       }
-      if constexpr (GROUPS > 1) {
-        float* mine = sm[warp][lane];
-        mine[0] = m0;
-        mine[1] = m1;
-        mine[2] = l0;
-        mine[3] = l1;
+      // the warps of a slice meet in a tree (blocks whose warps all have their own slice loop instead)
+      const int live = min(groups, w1 - w0 + 1);  // the others have nothing
+      for (int step = kJoinWarps / 2; step > 0; step >>= 1) {
+        if (step >= live) continue;
+        if (group >= step && group < 2 * step) {
+          float* mine = sm[warp][lane];
+          mine[0] = m0;
+          mine[1] = m1;
+          mine[2] = l0;
+          mine[3] = l1;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mine[4 + i] = o[i];
+          for (int i = 0; i < 4; ++i) mine[4 + i] = o[i];
+        }
         __syncthreads();
-        if (warp % GROUPS) return;
-        for (int w = warp + 1; w < warp + GROUPS; ++w) {
-          const float* x = sm[w][lane];
+        if (group < step && group + step < live) {
+          const float* x = sm[warp + step][lane];
           const float xo[4] = {x[4], x[5], x[6], x[7]};
           add(x[0], x[1], x[2], x[3], xo);
         }
       }
-      const int kvh = pc.hb / p.gblocks, g0 = (pc.hb - kvh * p.gblocks) * GB;
-      const int heads = min(GB, p.group - g0);
-      T* y = static_cast<T*>(p.y) + pc.s * p.y_seq + (long long)(kvh * p.group + g0) * p.y_head;
+      if (group == 0) {
+        const int kvh = hb / p.gblocks, g0 = (hb - kvh * p.gblocks) * GB;
+        const int heads = min(GB, p.group - g0);
+        T* y = static_cast<T*>(p.y) + s * p.y_seq + (long long)(kvh * p.group + g0) * p.y_head;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int h = C::k16 && (i & 1) ? h1 : h0;
-        if (h < heads && d[i] < p.c.dim) y[h * p.y_head + d[i]] = from_float<T>(o[i] / (C::k16 && (i & 1) ? l1 : l0));
+        for (int i = 0; i < 4; ++i) {
+          const int h = C::k16 && (i & 1) ? h1 : h0;
+          if (h < heads && d[i] < p.c.dim) y[h * p.y_head + d[i]] = from_float<T>(o[i] / (C::k16 && (i & 1) ? l1 : l0));
+        }
       }
     }
     return;
   }
   if constexpr (WTS) {
+    const int me = blockIdx.x;
     __shared__ float top[GB], inv[GB];
-    const int slice = blockIdx.y - 1, slices = gridDim.y - 1;
     for (int kind = 0; kind < 2; ++kind) {
       const Piece pc = p.pieces[me * 2 + kind];
       if (pc.s < 0) continue;
@@ -935,7 +975,6 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const _
         float m = kNothing, l = 0.0f;
         for (int w = pc.w0 + lane; w <= pc.w1; w += 32) {
           const int slot = w * 2 + (w == pc.w0 ? 1 : 0);
-          if (w != pc.w0 && p.pieces[slot].s < 0) continue;
           const float a = p.ml[(size_t)slot * 2 * GB + g], b = p.ml[(size_t)slot * 2 * GB + GB + g];
           const float t = fmaxf(m, a);
           l = l * exp2_from(m, t) + b * exp2_from(a, t);
@@ -956,11 +995,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const _
       __syncthreads();
       const float* win = p.win ? p.win + pc.s * p.win_seq + pc.hb * p.win_head : nullptr;
       float* wout = p.wout + pc.s * p.wout_seq + pc.hb * p.wout_head;
-      // this worker's tokens of the segment, dealt to the slices
+      // this worker's tokens of the segment
       const int t0 = (int)(pc.lo - pc.begin) * TK, t1 = min(len, (int)(pc.hi - pc.begin) * TK);
       constexpr int U = 4;  // tokens of a thread in flight
-      const int step = slices * kJoinWarps * 32;
-      for (int i0 = t0 + slice * kJoinWarps * 32 + tid; i0 < t1; i0 += U * step) {
+      constexpr int step = kJoinWarps * 32;
+      for (int i0 = t0 + tid; i0 < t1; i0 += U * step) {
         float w[U], sum[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -1011,6 +1050,8 @@ AttnPlan attention_plan_for(const AttnParams& p, int sms, bool weights) {
   pl.part = pl.whole ? 0 : up256((size_t)pl.workers * 2 * C::NR * 32 * 4);
   pl.ml = pl.whole ? 0 : up256((size_t)pl.workers * 2 * 2 * GB * 4);
   pl.pieces = pl.whole ? 0 : up256((size_t)pl.workers * 2 * sizeof(Piece));
+  pl.by_segment = segments * (C::NR / 4) <= 2 * sms;  // a block each in one round
+  pl.segs = pl.whole || !pl.by_segment ? 0 : up256((size_t)segments * sizeof(Segment));
   pl.lstride = C::k16 ? (p.group + 1) / 2 * 2 : p.group;
   pl.logits = weights ? up256((size_t)units * C::TK * pl.lstride * 4) : 0;
   return pl;
@@ -1042,12 +1083,15 @@ int attention_launch_for(AttnParams& p, const AttnPlan& pl, cudaStream_t st) {
   p.mode = attention_maps<C, T>(&p) ? kCopyTma : p.vec ? kCopyVec : kCopyElements;
   p.whole = pl.whole ? (p.capacity + C::TK - 1) / C::TK : 0;
   p.lstride = pl.lstride;
+  p.workers = pl.workers;
+  p.by_segment = !pl.whole && pl.by_segment;
   auto* kernel = attention_kernel<T, DPAD, GB, WTS>;
   SPINN_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
   const int rc = launch_dependent(kernel, dim3(pl.workers), kThreads, C::SMEM, st, p);
   if (rc || pl.whole) return rc;
-  return launch_dependent(attention_join_kernel<T, DPAD, GB, WTS>, dim3(pl.workers, WTS ? 2 : 1), kJoinWarps * 32, 0, st,
-                          p);
+  const int jobs = p.by_segment ? p.c.seqs * p.hblocks * (C::NR / 4) : pl.workers;
+  return launch_dependent(attention_join_kernel<T, DPAD, GB, WTS>, dim3((WTS ? pl.workers : 0) + jobs), kJoinWarps * 32, 0,
+                          st, p);
 }
 
 // The instantiation for a head size and group: `go` gets the Tile as a tag.

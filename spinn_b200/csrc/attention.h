@@ -17,6 +17,11 @@ struct Piece {
   unsigned begin, lo, hi;
 };
 
+// First and last worker of a segment, for a join by segments; w1 < 0: nothing to join.
+struct Segment {
+  int w0, w1;
+};
+
 enum AttnCopy { kCopyElements = 0, kCopyVec = 1, kCopyTma = 2 };
 
 struct AttnParams {
@@ -39,6 +44,9 @@ struct AttnParams {
   float* part;    // [worker][2][NR * 32] unnormalised outputs, in register order
   float* ml;      // [worker][2][2][GB] maxima and sums
   Piece* pieces;  // [worker][2]
+  Segment* segs;  // [sequence][head block], by_segment only
+  int workers;
+  bool by_segment;  // layout of the join
   float* logits;  // [unit][TK][lstride], scores in log2 units (weights only)
 };
 
@@ -46,7 +54,8 @@ struct AttnParams {
 struct AttnPlan {
   bool whole;  // one CTA per (sequence, head block), nothing to join
   int workers, lstride;
-  size_t part, ml, pieces, logits;
+  bool by_segment;
+  size_t part, ml, pieces, segs, logits;
 };
 
 inline size_t up256(size_t b) { return (b + 255) & ~size_t(255); }
