@@ -45,7 +45,7 @@ constexpr int kWholeTiles = 8;  // longest cache, in tiles, that is left to one 
 constexpr uint64_t kTimeoutNs = 4000000000ull, kDrainNs = 200000000ull;  // bounded barrier waits
 
 // Tile shapes.  GB: heads of one block (8 or 16 with 16-bit types, where they are the columns of
-// an MMA; up to 8 with fp32).  DPAD: head_dim padded to the next instantiated size.
+// an MMA; 1, 4 or 8 with fp32).  DPAD: head_dim padded to the next instantiated size.
 template <typename T, int DPAD_, int GB_>
 struct Tile {
   static constexpr int DPAD = DPAD_, GB = GB_;
@@ -63,7 +63,8 @@ struct Tile {
   static constexpr int MLR = k16 ? GB / 8 * 2 : GB;  // heads whose state a lane holds
   static constexpr int DUMP = (NR + 2 * MLR) * 32 * 4;
   static constexpr int EXTRA = 2 * DUMP + (k16 ? 0 : GB * DPAD * 4) + 2 * GB * 4 + 64 + kWarps * 6 * 8 + 16 + 1024;
-  // Two CTAs per SM where three stages fit in half of the shared memory, else one
+  // Two CTAs per SM where three stages fit in half of the shared memory, else one (three and four
+  // CTAs measured no faster)
   static constexpr int kHalfSm = 113 * 1024, kSm = 226 * 1024;
   static constexpr int FIT2 = (kHalfSm - EXTRA) / STAGE, FIT1 = (kSm - EXTRA) / STAGE;
   static constexpr int CTAS = FIT2 >= 3 ? 2 : 1;
@@ -1109,6 +1110,13 @@ auto attention_dispatch(int dim, int group, F go) {
     if (dim <= 64) return go(Tile<T, 64, SMALL>());
     if (dim <= 128) return go(Tile<T, 128, SMALL>());
     return go(Tile<T, 256, SMALL>());
+  }
+  if constexpr (sizeof(T) == 4) {
+    if (group <= 4) {
+      if (dim <= 64) return go(Tile<T, 64, 4>());
+      if (dim <= 128) return go(Tile<T, 128, 4>());
+      return go(Tile<T, 256, 4>());
+    }
   }
   if (dim <= 64) return go(Tile<T, 64, LARGE>());
   if (dim <= 128) return go(Tile<T, 128, LARGE>());
