@@ -206,7 +206,8 @@ int spinn_cuda_cache_append(const SpinnCudaCache *cache, const SpinnCudaPageTabl
  * weights_out, when not NULL ([seqs][kv_heads][>= lens[s]] fp32, group <= 16, weights_capacity
  * entries per row): weights_out[s][j][t] = weights_in[s][j][t] + the sum of p[s][h][t] over the
  * heads h of group j, for t < lens[s]; entries beyond are left as they were.  weights_in NULL
- * counts as zeros; it may be weights_out itself. */
+ * counts as zeros; it may be weights_out itself, and may not overlap it otherwise.  Cached keys or
+ * values that are not finite make the outputs that read them so. */
 typedef struct {
     const void *q;
     void *y;
@@ -232,7 +233,7 @@ int spinn_cuda_paged_attention(const SpinnCudaCache *cache, const SpinnCudaPageT
  * beyond are left as they were).  new_lens[s] = n.
  * out_pages == the table's pages (the same pointer): in place; then no page may belong to two
  * sequences, and out_row_stride is the table's.  Otherwise out_pages names pages that no
- * sequence of the call reads, enough for n tokens per row.  weights_out may be weights_in. */
+ * sequence of the call reads, no page twice, enough for n tokens per row.  weights_out may be weights_in. */
 typedef struct {
     const float *weights_in;
     float *weights_out;

@@ -10,8 +10,8 @@
 // dealt to a fixed number of CTAs in equal contiguous shares, whatever the lengths; every CTA
 // finds its share from the lengths on the device, so the host needs to know none of them and a
 // ragged batch is as balanced as an even one.  A (sequence, head) that lies in one share is
-// finished there; one that crosses shares leaves a partial result per share (running maximum,
-// sum and unnormalised output), and the second kernel joins them.
+// finished there; one that crosses shares leaves a partial result per share (running
+// reference, sum and unnormalised output), and the second kernel joins them.
 //
 // A batch whose caches are all short (the table holds at most eight tiles, and there is an SM slot
 // for every (sequence, head)) is not split: each CTA takes one (sequence, head) and there is
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
     uint8_t* tile = ring + stage * C::STAGE;
     if (mode == kCopyTma) {
       if (!mbar_wait(&full[stage], phases >> stage & 1, abort_flag, kTimeoutNs)) {
-        if (lane == 0) atomicOr(p.c.err, kLinearTimeout);
+        if (lane == 0) atomicOr(p.c.err, kWaitExpired);
       }
       phases ^= 1u << stage;
       if (left < RW) {

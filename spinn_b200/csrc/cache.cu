@@ -763,7 +763,7 @@ __attribute__((visibility("default"))) int spinn_cuda_stream_sync(void* stream) 
   if (!bits) return 0;
   SPINN_CUDA_TRY(cudaMemsetAsync(word, 0, sizeof(bits), st));
   SPINN_CUDA_TRY(cudaStreamSynchronize(st));
-  if (bits & kLinearTimeout) {
+  if (bits & kWaitExpired) {
     set_error("a kernel's bounded wait expired");
     return SPINN_CUDA_ETIMEOUT;
   }

@@ -12,7 +12,7 @@ namespace spinn {
 
 // Deferred errors of the decoder-serving operators, raised by a kernel that skips the access instead of
 // making it (spinn_cuda_stream_sync reports and clears them).
-enum CacheErr : unsigned { kCacheBadPage = 1, kCacheBadLength = 2, kCacheSamePage = 4, kLinearTimeout = 8 };
+enum DecodeErr : unsigned { kCacheBadPage = 1, kCacheBadLength = 2, kCacheSamePage = 4, kWaitExpired = 8 };
 
 // The pools and their page table as the kernels see them.  Strides are in elements.
 struct CacheView {
@@ -66,7 +66,7 @@ int check_stream_device(const char* who, void* stream, int* device);
 bool cache_vec16(const CacheView& v, int bytes);
 int dtype_bytes(int dtype);
 
-// The current device's deferred error word (device memory; CacheErr bits, kLinearTimeout).
+// The current device's deferred error word (device memory; DecodeErr bits).
 int decode_error_word(int device, unsigned** word);
 
 }  // namespace spinn

@@ -746,7 +746,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
   __syncthreads();
   if constexpr (PAIR == 2) cluster_sync();  // no CTA leaves while its peer may use its memory
-  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.err, kLinearTimeout);
+  if (threadIdx.x == 0 && *abort_flag) atomicOr(p.err, kWaitExpired);
   if (warp == 2) {
     tc_fence_after();
     if constexpr (PAIR == 2)

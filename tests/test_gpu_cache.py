@@ -265,16 +265,19 @@ FIRST_CALLS = """
 import torch
 from spinn_b200 import runtime as rt
 dt = torch.bfloat16
-k = torch.randn(40, 16, 2, 64, device="cuda").to(dt); v = k.clone()
-table = torch.arange(40, dtype=torch.int32, device="cuda").view(2, 20); lens = torch.tensor([100, 7], dtype=torch.int32, device="cuda")
+k = torch.randn(800, 16, 2, 64, device="cuda").to(dt); v = k.clone()
+table = torch.arange(800, dtype=torch.int32, device="cuda").view(2, 400); lens = torch.tensor([100, 7], dtype=torch.int32, device="cuda")
 q = torch.randn(2, 8, 64, device="cuda").to(dt); y = torch.empty_like(q)
-w = torch.zeros(2, 2, 320, device="cuda"); new = torch.empty(2, dtype=torch.int32, device="cuda")
+w = torch.zeros(2, 2, 6400, device="cuda"); new = torch.empty(2, dtype=torch.int32, device="cuda")
 kept = torch.empty(2, 2, 50, dtype=torch.int32, device="cuda")
 row = torch.randn(2, 2, 64, device="cuda").to(dt)
 x = torch.randn(40, 65, device="cuda").to(dt); m = torch.randn(32, 65, device="cuda").to(dt); z = torch.empty(40, 32, device="cuda").to(dt)
+big = torch.randn(64, 2048, device="cuda").to(dt); wide = torch.randn(1000, 2048, device="cuda").to(dt)
+split = torch.empty(64, 1000, device="cuda").to(dt)
 torch.cuda.synchronize()
 g = torch.cuda.CUDAGraph()
 with torch.cuda.graph(g):
+    rt.linear(big, wide, split)
     rt.cache_append(row, row, k, v, table, lens)
     rt.paged_attention(q, k, v, table, lens, y, None, w, w)
     rt.linear(x, m, z)
@@ -283,6 +286,7 @@ with torch.cuda.graph(g):
 g.replay()
 rt.stream_sync()
 assert new.tolist() == [50, 7] and abs(float(w[1].sum()) - 8) < 1e-4 and torch.isfinite(z.float()).all()
+assert (split.float() - big.float() @ wide.float().T).abs().max() < 1.0
 print("replayed")
 """
 
