@@ -63,11 +63,12 @@ struct Tile {
   static constexpr int MLR = k16 ? GB / 8 * 2 : GB;  // heads whose state a lane holds
   static constexpr int DUMP = (NR + 2 * MLR) * 32 * 4;
   static constexpr int EXTRA = 2 * DUMP + (k16 ? 0 : GB * DPAD * 4) + 2 * GB * 4 + 64 + kWarps * 6 * 8 + 16 + 1024;
-  // Two CTAs per SM where three stages fit in half of the shared memory, else one (three and four
-  // CTAs measured no faster)
+  // Two CTAs per SM where three stages fit in half of the shared memory (two, for 16-bit rows of 192:
+  // 32 x 8192 takes 159 us, 193 padded to 256 with one CTA), else one; three and four CTAs measured no
+  // faster.
   static constexpr int kHalfSm = 113 * 1024, kSm = 226 * 1024;
   static constexpr int FIT2 = (kHalfSm - EXTRA) / STAGE, FIT1 = (kSm - EXTRA) / STAGE;
-  static constexpr int CTAS = FIT2 >= 3 ? 2 : 1;
+  static constexpr int CTAS = FIT2 >= (DPAD == 192 ? 2 : 3) ? 2 : 1;
   static constexpr int NS = CTAS == 2 ? (FIT2 > 6 ? 6 : FIT2) : (FIT1 > 6 ? 6 : FIT1);
   static constexpr int SMEM = NS * STAGE + EXTRA;
   static_assert(NS >= 2, "pipeline needs two stages");
@@ -1106,21 +1107,20 @@ int attention_launch_for(AttnParams& p, const AttnPlan& pl, cudaStream_t st) {
 template <typename T, typename F>
 auto attention_dispatch(int dim, int group, F go) {
   constexpr int SMALL = sizeof(T) == 2 ? 8 : 1, LARGE = sizeof(T) == 2 ? 16 : 8;
-  if (group <= SMALL) {
-    if (dim <= 64) return go(Tile<T, 64, SMALL>());
-    if (dim <= 128) return go(Tile<T, 128, SMALL>());
-    return go(Tile<T, 256, SMALL>());
-  }
-  if constexpr (sizeof(T) == 4) {
-    if (group <= 4) {
-      if (dim <= 64) return go(Tile<T, 64, 4>());
-      if (dim <= 128) return go(Tile<T, 128, 4>());
-      return go(Tile<T, 256, 4>());
+  auto by_dim = [&](auto gb) {
+    constexpr int GB = decltype(gb)::value;
+    if (dim <= 64) return go(Tile<T, 64, GB>());
+    if (dim <= 128) return go(Tile<T, 128, GB>());
+    if constexpr (sizeof(T) == 2) {
+      if (dim <= 192) return go(Tile<T, 192, GB>());
     }
+    return go(Tile<T, 256, GB>());
+  };
+  if (group <= SMALL) return by_dim(std::integral_constant<int, SMALL>());
+  if constexpr (sizeof(T) == 4) {
+    if (group <= 4) return by_dim(std::integral_constant<int, 4>());
   }
-  if (dim <= 64) return go(Tile<T, 64, LARGE>());
-  if (dim <= 128) return go(Tile<T, 128, LARGE>());
-  return go(Tile<T, 256, LARGE>());
+  return by_dim(std::integral_constant<int, LARGE>());
 }
 
 template <typename T>
