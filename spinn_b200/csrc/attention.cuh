@@ -50,7 +50,9 @@ template <typename T, int DPAD_, int GB_>
 struct Tile {
   static constexpr int DPAD = DPAD_, GB = GB_;
   static constexpr bool k16 = sizeof(T) == 2;
-  static constexpr int RW = k16 ? 16 : 8;   // tokens of a warp
+  // Tokens of a warp.  What a tile costs beside its bytes (fetching, waiting, the softmax's chain) makes
+  // 16 the better number wherever two CTAs still fit (64 x 4096 fp32 of 64: 128 us with 8, 98 with 16).
+  static constexpr int RW = k16 || DPAD <= 96 ? 16 : 8;
   static constexpr int TK = RW * kWarps;    // tokens of a unit
   static constexpr int CH = DPAD * sizeof(T) / 16;  // 16-byte chunks of a row
   // 16-bit rows lie in sub-tiles of 128 bytes a row, chunk c at c ^ (row % 8): the TMA's 128-byte
@@ -63,12 +65,12 @@ struct Tile {
   static constexpr int MLR = k16 ? GB / 8 * 2 : GB;  // heads whose state a lane holds
   static constexpr int DUMP = (NR + 2 * MLR) * 32 * 4;
   static constexpr int EXTRA = 2 * DUMP + (k16 ? 0 : GB * DPAD * 4) + 2 * GB * 4 + 64 + kWarps * 6 * 8 + 16 + 1024;
-  // Two CTAs per SM where three stages fit in half of the shared memory (two, for 16-bit rows of 192:
-  // 32 x 8192 takes 159 us, 193 padded to 256 with one CTA), else one; three and four CTAs measured no
-  // faster.
+  // Two CTAs per SM where three stages fit in half of the shared memory (two stages, for rows of 384
+  // bytes: 32 x 8192 16-bit of 192 takes 159 us, 193 padded to 256 with one CTA), else one; three and
+  // four CTAs measured no faster.
   static constexpr int kHalfSm = 113 * 1024, kSm = 226 * 1024;
   static constexpr int FIT2 = (kHalfSm - EXTRA) / STAGE, FIT1 = (kSm - EXTRA) / STAGE;
-  static constexpr int CTAS = FIT2 >= (DPAD == 192 ? 2 : 3) ? 2 : 1;
+  static constexpr int CTAS = FIT2 >= (CH == 24 ? 2 : 3) ? 2 : 1;
   static constexpr int NS = CTAS == 2 ? (FIT2 > 6 ? 6 : FIT2) : (FIT1 > 6 ? 6 : FIT1);
   static constexpr int SMEM = NS * STAGE + EXTRA;
   static_assert(NS >= 2, "pipeline needs two stages");
@@ -622,11 +624,14 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
     } else {
       // fp32 on the FMA units: lane = (token of eight, quarter of the row) for the scores, a
       // chunk of four output dims for the products
+      constexpr int RB = RW / 8;  // tokens of a lane
       const float4* q4 = reinterpret_cast<const float4*>(qs);
       const int key = lane >> 2, part = lane & 3;
-      float s[GB];
+      float s[RB][GB];
 #pragma unroll
-      for (int g = 0; g < GB; ++g) s[g] = 0.0f;
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int g = 0; g < GB; ++g) s[b][g] = 0.0f;
       // Four lanes to a token take every fourth chunk.  Where rows start on the same banks, odd tokens
       // take the chunks of a pair of steps in the other order: all eight groups of banks at once.
       const int chunks = (p.c.dim + 3) >> 2;
@@ -635,28 +640,37 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
       for (int i = 0; i < chunks; i += 4) {
         const int ch = i + part < chunks && (i ^ flip) + part < chunks ? (i ^ flip) + part : i + part;
         if (ch >= chunks) continue;
-        const float4 x = *reinterpret_cast<const float4*>(tile + chunk_at(key, ch));
+        float4 x[RB];
+#pragma unroll
+        for (int b = 0; b < RB; ++b) x[b] = *reinterpret_cast<const float4*>(tile + chunk_at(key + 8 * b, ch));
 #pragma unroll
         for (int g = 0; g < GB; ++g) {
           const float4 y = q4[g * (DPAD / 4) + ch];
-          s[g] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[g]))));
+#pragma unroll
+          for (int b = 0; b < RB; ++b)
+            s[b][g] = fmaf(x[b].x, y.x, fmaf(x[b].y, y.y, fmaf(x[b].z, y.z, fmaf(x[b].w, y.w, s[b][g]))));
         }
       }
       bool grew = false;
 #pragma unroll
-      for (int g = 0; g < GB; ++g) {
-        s[g] += __shfl_xor_sync(0xffffffffu, s[g], 1);
-        s[g] += __shfl_xor_sync(0xffffffffu, s[g], 2);
-        s[g] = key < left ? s[g] * p.scale_log2 : -INFINITY;
-        grew |= s[g] - m[g] > 8.0f;
-        if constexpr (WTS) {
-          if (part == 0 && key < left && g < p.lstride) p.logits[((long long)unit * TK + warp * RW + key) * p.lstride + g] = s[g];
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int g = 0; g < GB; ++g) {
+          float& v = s[b][g];
+          v += __shfl_xor_sync(0xffffffffu, v, 1);
+          v += __shfl_xor_sync(0xffffffffu, v, 2);
+          v = key + 8 * b < left ? v * p.scale_log2 : -INFINITY;
+          grew |= v - m[g] > 8.0f;
+          if constexpr (WTS) {
+            if (part == 0 && key + 8 * b < left && g < p.lstride)
+              p.logits[((long long)unit * TK + warp * RW + key + 8 * b) * p.lstride + g] = v;
+          }
         }
-      }
       if (__any_sync(0xffffffffu, grew)) {  // as above
 #pragma unroll
         for (int g = 0; g < GB; ++g) {
-          float x = s[g];
+          float x = s[0][g];
+          if constexpr (RB > 1) x = fmaxf(x, s[RB - 1][g]);
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -669,10 +683,12 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
         }
       }
 #pragma unroll
-      for (int g = 0; g < GB; ++g) {
-        s[g] = exp2_from(s[g], m[g]);
-        l[g] += s[g];
-      }
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int g = 0; g < GB; ++g) {
+          s[b][g] = exp2_from(s[b][g], m[g]);
+          l[g] += s[b][g];
+        }
 #pragma unroll
       for (int r = 0; r < RW; ++r) {
 #pragma unroll
@@ -682,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
                                       : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
           for (int g = 0; g < GB; ++g) {
-            const float w = __shfl_sync(0xffffffffu, s[g], r * 4);
+            const float w = __shfl_sync(0xffffffffu, s[r / 8][g], r % 8 * 4);
             float(&acc)[4] = o[g * C::CPL + ci];
             acc[0] = fmaf(w, x.x, acc[0]);
             acc[1] = fmaf(w, x.y, acc[1]);
@@ -1110,6 +1126,9 @@ auto attention_dispatch(int dim, int group, F go) {
   auto by_dim = [&](auto gb) {
     constexpr int GB = decltype(gb)::value;
     if (dim <= 64) return go(Tile<T, 64, GB>());
+    if constexpr (sizeof(T) == 4) {
+      if (dim <= 96) return go(Tile<T, 96, GB>());
+    }
     if (dim <= 128) return go(Tile<T, 128, GB>());
     if constexpr (sizeof(T) == 2) {
       if (dim <= 192) return go(Tile<T, 192, GB>());
