@@ -149,8 +149,10 @@ int spinn_cuda_conv2d_noalloc(const float *x, const float *w, const float *bias,
  * stream) must belong to the current device; nothing is waited for and nothing is allocated, so
  * calls may be captured into CUDA graphs.  A call that needs a workspace takes it from the
  * caller (the _workspace function gives its size, 16-byte aligned, contents irrelevant before
- * and after); two calls that may overlap on the GPU need two workspaces.  Arguments are checked
- * before any work is queued (SPINN_CUDA_EINVAL).  What only the device can see -- a page number
+ * and after); two calls that may overlap on the GPU need two workspaces.  What a call writes has
+ * rows apart from one another and from what it reads, but where an operator says otherwise.  Sizes
+ * and lengths are at most 2^31 - 65536.  Arguments are checked before any work is queued
+ * (SPINN_CUDA_EINVAL).  What only the device can see -- a page number
  * outside the pool, a length beyond the table -- is skipped by the kernel without touching
  * memory, and reported by the next spinn_cuda_stream_sync. */
 
@@ -161,7 +163,7 @@ int spinn_cuda_conv2d_noalloc(const float *x, const float *w, const float *bias,
 
 /* Waits for `stream` and returns (and clears) the deferred error of the operators below on the
  * current device: SPINN_CUDA_EINVAL for a bad page or length, SPINN_CUDA_ETIMEOUT for an
- * expired wait.  Not during capture. */
+ * expired wait.  Refused while `stream` is being captured. */
 int spinn_cuda_stream_sync(void *stream);
 
 /* Two page pools of one shape: keys and values, [num_pages][page_size][kv_heads][head_dim] with
@@ -274,6 +276,11 @@ int spinn_cuda_linear(const SpinnCudaLinear *l, void *workspace, size_t workspac
  * row. */
 int64_t spinn_cuda_diag_cache_slot(const int32_t *row, int max_pages, int pos, int page_size, int num_pages,
                                    int64_t page_stride, int64_t token_stride);
+/* Diagnostics (host only): two operands as {address, bytes per element, elements per row, three
+ * counts of rows, their three strides in elements}: bit 0 of the result when no two rows of `a`
+ * share an element, bit 1 when `a` and `b` share none (clear also where that is not known: see
+ * csrc/cache.h). */
+int spinn_cuda_diag_rows(const int64_t *a, const int64_t *b);
 /* Diagnostics (host only): attention's split of `units` tiles over `workers`: out3 = {first unit
  * of `worker`, its end, the worker that owns `unit`}. */
 int spinn_cuda_diag_attention_share(int64_t units, int workers, int worker, int64_t unit, int64_t *out3);

@@ -103,6 +103,19 @@ __attribute__((visibility("default"))) int spinn_cuda_paged_attention(const Spin
   const size_t need = pl.part + pl.ml + pl.pieces + pl.segs + pl.logits;
   SPINN_CHECK_ARG(!need || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
                   "paged_attention: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
+  const int es = dtype_bytes(cache->dtype);
+  const Rows q = {a->q, es, cache->head_dim, {table->seqs, a->q_heads, 1}, {a->q_seq_stride, a->q_head_stride, 0}};
+  const Rows y = {a->y, es, cache->head_dim, {table->seqs, a->q_heads, 1}, {a->y_seq_stride, a->y_head_stride, 0}};
+  SPINN_CHECK_ARG(rows_distinct(y) && rows_apart(y, q), "paged_attention: rows of y overlap one another or q");
+  if (a->weights_out) {
+    const Rows wout = {a->weights_out, 4, a->weights_capacity, {table->seqs, cache->kv_heads, 1},
+                       {a->wout_seq_stride, a->wout_head_stride, 0}};
+    const Rows win = {a->weights_in, 4, a->weights_capacity, {table->seqs, cache->kv_heads, 1},
+                      {a->win_seq_stride, a->win_head_stride, 0}};
+    SPINN_CHECK_ARG(rows_distinct(wout), "paged_attention: rows of weights_out overlap");
+    SPINN_CHECK_ARG(!a->weights_in || a->weights_in == a->weights_out || rows_apart(wout, win),
+                    "paged_attention: weights_out must be weights_in itself or apart from it");
+  }
   char* ws = static_cast<char*>(workspace);
   p.part = reinterpret_cast<float*>(ws);
   p.ml = reinterpret_cast<float*>(ws + pl.part);

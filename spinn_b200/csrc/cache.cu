@@ -1,8 +1,7 @@
 // cache.cu -- the paged key-value cache: host checks shared by its entry points, appending new
 // tokens, and eviction by accumulated attention weight.  Attention itself is in attention.cu.
 #include <algorithm>
-#include <map>
-#include <mutex>
+#include <atomic>
 
 #include "cache.h"
 #include "internal.h"
@@ -11,27 +10,30 @@
 
 namespace spinn {
 
+constexpr int kMaxDevices = 64;
+
 // One word per device, in the library's own image: no allocation, so that a first call may be a
 // captured one.
 __device__ unsigned g_decode_err = 0;
 
 int decode_error_word(int device, unsigned** word) {
-  static std::mutex mu;
-  static std::map<int, unsigned*> addr;
-  std::lock_guard<std::mutex> lk(mu);
-  unsigned*& a = addr[device];
-  if (!a) {
-    void* p = nullptr;
-    SPINN_CUDA_TRY(cudaGetSymbolAddress(&p, g_decode_err));
-    a = static_cast<unsigned*>(p);
-  }
-  *word = a;
+  static std::atomic<unsigned*> addr[kMaxDevices];
+  SPINN_CHECK_ARG(device >= 0 && device < kMaxDevices, "device %d is past the %d supported", device, kMaxDevices);
+  *word = addr[device].load();
+  if (*word) return 0;
+  void* p = nullptr;
+  SPINN_CUDA_TRY(cudaGetSymbolAddress(&p, g_decode_err));
+  *word = static_cast<unsigned*>(p);
+  addr[device].store(*word);
   return 0;
 }
 
 int dtype_bytes(int dtype) {
   return dtype == SPINN_CUDA_FP32 ? 4 : (dtype == SPINN_CUDA_FP16 || dtype == SPINN_CUDA_BF16) ? 2 : 0;
 }
+
+// Clears what has been reported, and no more: another stream's kernel may raise an error meanwhile.
+__global__ void clear_errors_kernel(unsigned* word, unsigned bits) { atomicAnd(word, ~bits); }
 
 int check_stream_device(const char* who, void* stream, int* device) {
   SPINN_CUDA_TRY(cudaGetDevice(device));
@@ -85,6 +87,43 @@ bool cache_vec16(const CacheView& v, int bytes) {
   const int per = 16 / bytes;
   return aligned16(v.k) && aligned16(v.v) && v.dim % per == 0 && v.page_stride % per == 0 &&
          v.token_stride % per == 0 && v.head_stride % per == 0;
+}
+
+namespace {
+
+// Extents of nested rows in bytes: of all of them, of one step of the outermost dimension, and
+// that dimension's stride (0: a single row).
+struct Extent {
+  long long all, inner, stride;
+  bool nested;
+};
+
+Extent extent(const Rows& r) {
+  int order[3] = {0, 1, 2};
+  std::sort(order, order + 3, [&](int a, int b) { return r.stride[a] < r.stride[b]; });
+  Extent e = {r.width * r.bytes, r.width * r.bytes, 0, true};
+  for (int i : order) {
+    if (r.count[i] <= 1) continue;
+    e.stride = r.stride[i] * r.bytes;
+    e.inner = e.all;
+    e.nested &= e.stride >= e.all;
+    e.all += (r.count[i] - 1) * e.stride;
+  }
+  return e;
+}
+
+}  // namespace
+
+bool rows_distinct(const Rows& r) { return extent(r).nested; }
+
+bool rows_apart(const Rows& a, const Rows& b) {
+  const Extent x = extent(a), y = extent(b);
+  const long long d = (long long)((uintptr_t)b.p - (uintptr_t)a.p);
+  if (d >= x.all || -d >= y.all) return true;
+  const long long s = x.stride ? x.stride : y.stride;
+  if (!s || !x.nested || !y.nested || (x.stride && y.stride && x.stride != y.stride)) return false;
+  const long long at = (d % s + s) % s;
+  return at >= x.inner && at + y.inner <= s;
 }
 
 namespace {
@@ -712,10 +751,8 @@ __global__ void __launch_bounds__(256) evict_shift_kernel(const EvictParams p, i
 // Clusters of 1 .. 8 CTAs of the selection kernel, at their largest, that the device holds at once
 // (its GPCs do not divide evenly: 15 of eight, 22 of six, 26 of five on 148 SMs).
 int select_clusters(int device, int ctas) {
-  static std::mutex mu;
-  static std::map<std::pair<int, int>, int> known;
-  std::lock_guard<std::mutex> lk(mu);
-  int& n = known[{device, ctas}];
+  static std::atomic<int> known[kMaxDevices][9];  // ctas <= 8
+  int n = known[device][ctas].load();
   if (!n) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
@@ -732,6 +769,7 @@ int select_clusters(int device, int ctas) {
       cudaGetLastError();
       n = 1;
     }
+    known[device][ctas].store(n);
   }
   return n;
 }
@@ -768,6 +806,13 @@ int launch_select(const EvictParams& p, int pairs, int device, cudaStream_t st) 
   return 0;
 }
 
+// Pools that are written: two of them, and no row twice.
+bool pools_distinct(const SpinnCudaCache& c, int bytes) {
+  const Rows k = {c.k, bytes, c.head_dim, {c.num_pages, c.page_size, c.kv_heads},
+                  {c.page_stride, c.token_stride, c.head_stride}};
+  return rows_distinct(k) && c.k != c.v;
+}
+
 bool overlap(const void* a, size_t na, const void* b, size_t nb) {
   const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
   return x < y + nb && y < x + na;
@@ -785,11 +830,15 @@ __attribute__((visibility("default"))) int spinn_cuda_stream_sync(void* stream) 
   rc = decode_error_word(dev, &word);
   if (rc) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  SPINN_CUDA_TRY(cudaStreamIsCapturing(st, &cap));
+  SPINN_CHECK_ARG(cap == cudaStreamCaptureStatusNone, "stream_sync: the stream is being captured");
   unsigned bits = 0;
   SPINN_CUDA_TRY(cudaMemcpyAsync(&bits, word, sizeof(bits), cudaMemcpyDeviceToHost, st));
   SPINN_CUDA_TRY(cudaStreamSynchronize(st));
   if (!bits) return 0;
-  SPINN_CUDA_TRY(cudaMemsetAsync(word, 0, sizeof(bits), st));
+  clear_errors_kernel<<<1, 1, 0, st>>>(word, bits);
+  SPINN_CUDA_TRY(cudaGetLastError());
   SPINN_CUDA_TRY(cudaStreamSynchronize(st));
   if (bits & kWaitExpired) {
     set_error("a kernel's bounded wait expired");
@@ -823,6 +872,8 @@ __attribute__((visibility("default"))) int spinn_cuda_cache_append(const SpinnCu
   if (rows->tokens == 0) return 0;
   rc = decode_error_word(dev, &p.c.err);
   if (rc) return rc;
+  SPINN_CHECK_ARG(pools_distinct(*cache, es), "cache_append: the pools' rows overlap");
+  SPINN_CHECK_ARG(rows->tokens <= kMaxLength, "cache_append: %d tokens", rows->tokens);
   p.k = rows->k;
   p.v = rows->v;
   p.k_tok = rows->k_token_stride;
@@ -852,7 +903,8 @@ __attribute__((visibility("default"))) int spinn_cuda_cache_evict(const SpinnCud
   if (rc) return rc;
   SPINN_CHECK_ARG(e && e->weights_in && e->weights_out && e->out_pages && e->new_lens && e->kept,
                   "cache_evict: weights, out_pages, new_lens and kept are required");
-  SPINN_CHECK_ARG(e->budget > 0 && e->recent >= 0, "cache_evict: budget %d, recent %d", e->budget, e->recent);
+  SPINN_CHECK_ARG(e->budget > 0 && e->budget <= kMaxLength && e->recent >= 0, "cache_evict: budget %d, recent %d",
+                  e->budget, e->recent);
   SPINN_CHECK_ARG(e->out_max_pages > 0 && e->out_row_stride >= 0 && e->weights_capacity > 0,
                   "cache_evict: bad output table or weights");
   SPINN_CHECK_ARG(e->win_seq_stride >= 0 && e->win_head_stride >= 0 && e->wout_seq_stride >= 0 &&
@@ -865,7 +917,7 @@ __attribute__((visibility("default"))) int spinn_cuda_cache_evict(const SpinnCud
   const long long pairs = (long long)table->seqs * cache->kv_heads;
   SPINN_CHECK_ARG(pairs <= 65535, "cache_evict: %lld (sequence, head) pairs, at most 65535", pairs);
   p.in_place = e->out_pages == table->pages;
-  SPINN_CHECK_ARG(!p.in_place || e->out_row_stride == table->row_stride,
+  SPINN_CHECK_ARG(!p.in_place || table->seqs == 1 || e->out_row_stride == table->row_stride,
                   "cache_evict: in place, the output table's stride must be the table's");
   p.same_weights = e->weights_in == e->weights_out;
   const size_t wi = 4 * ((table->seqs - 1) * (size_t)e->win_seq_stride + (cache->kv_heads - 1) * (size_t)e->win_head_stride +
@@ -880,6 +932,11 @@ __attribute__((visibility("default"))) int spinn_cuda_cache_evict(const SpinnCud
   if (rc) return rc;
   rc = decode_error_word(dev, &p.c.err);
   if (rc) return rc;
+  const int es = dtype_bytes(cache->dtype);
+  SPINN_CHECK_ARG(pools_distinct(*cache, es), "cache_evict: the pools' rows overlap");
+  const Rows weights = {e->weights_out, 4, e->weights_capacity, {table->seqs, cache->kv_heads, 1},
+                        {e->wout_seq_stride, e->wout_head_stride, 0}};
+  SPINN_CHECK_ARG(rows_distinct(weights), "cache_evict: rows of weights_out overlap");
   p.win = e->weights_in;
   p.wout = e->weights_out;
   p.win_seq = e->win_seq_stride;
@@ -889,7 +946,7 @@ __attribute__((visibility("default"))) int spinn_cuda_cache_evict(const SpinnCud
   p.out_table = e->out_pages;
   p.out_stride = e->out_row_stride;
   p.out_pages = e->out_max_pages;
-  p.wcap = e->weights_capacity;
+  p.wcap = std::min(e->weights_capacity, kMaxLength);
   p.new_lens = e->new_lens;
   p.kept = e->kept;
   p.budget = e->budget;
@@ -897,7 +954,6 @@ __attribute__((visibility("default"))) int spinn_cuda_cache_evict(const SpinnCud
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   rc = launch_select(p, (int)pairs, dev, st);
   if (rc) return rc;
-  const int es = dtype_bytes(cache->dtype);
   const bool vec = cache_vec16(p.c, es);
   const int units = vec ? p.c.dim * es / 16 : p.c.dim;  // copied units of a row
   if (p.in_place) {
@@ -922,6 +978,14 @@ __attribute__((visibility("default"))) int64_t spinn_cuda_diag_cache_slot(const 
                                                                           int64_t page_stride, int64_t token_stride) {
   if (!row || max_pages <= 0 || page_size <= 0 || pos < 0 || pos >= cache_capacity(max_pages, page_size)) return -2;
   return cache_slot(row, pos, page_size, num_pages, page_stride, token_stride);
+}
+
+__attribute__((visibility("default"))) int spinn_cuda_diag_rows(const int64_t* a, const int64_t* b) {
+  SPINN_CHECK_ARG(a && b, "diag_rows: two operands are required");
+  const auto rows = [](const int64_t* r) {
+    return Rows{(const void*)(uintptr_t)r[0], (int)r[1], r[2], {r[3], r[4], r[5]}, {r[6], r[7], r[8]}};
+  };
+  return (rows_distinct(rows(a)) ? 1 : 0) | (rows_apart(rows(a), rows(b)) ? 2 : 0);
 }
 
 __attribute__((visibility("default"))) int spinn_cuda_diag_attention_share(int64_t units, int workers, int worker,

@@ -27,10 +27,13 @@ struct CacheView {
   unsigned* err;  // deferred error word of the device
 };
 
-// Tokens that a table row can hold (lengths are 32-bit).
+// Sizes and lengths end 65536 before 2^31: indices in 32 bits step past their end by a tile.
+constexpr int kMaxLength = 0x7fff0000;
+
+// Tokens that a table row can hold.
 __host__ __device__ inline int cache_capacity(int max_pages, int page_size) {
   const long long c = (long long)max_pages * page_size;
-  return c > 0x7fffffffLL ? 0x7fffffff : (int)c;
+  return c > kMaxLength ? kMaxLength : (int)c;
 }
 
 // Element offset of token `pos` in either pool (head 0) through the table row `row`, or -1 when
@@ -65,6 +68,21 @@ int check_stream_device(const char* who, void* stream, int* device);
 // 16-byte vector access possible: `bytes`-sized elements, pointers and strides (elements).
 bool cache_vec16(const CacheView& v, int bytes);
 int dtype_bytes(int dtype);
+
+// What an operand covers: rows of `width` elements of `bytes` each, count[i] of them at stride[i]
+// (elements, >= 0) along up to three dimensions.
+struct Rows {
+  const void* p;
+  int bytes;
+  long long width;
+  long long count[3], stride[3];
+};
+// No two rows share an element (a tensor that is written must not: its rows are written by many
+// CTAs).  Dimensions nest, in any order.
+bool rows_distinct(const Rows& r);
+// No element of `a` is one of `b`.  Operands that interleave in one buffer (slices of its rows)
+// are told apart when their outermost strides agree.
+bool rows_apart(const Rows& a, const Rows& b);
 
 // The current device's deferred error word (device memory; DecodeErr bits).
 int decode_error_word(int device, unsigned** word);

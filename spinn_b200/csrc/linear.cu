@@ -901,7 +901,8 @@ int linear_params(const SpinnCudaLinear* l, LinearParams* p) {
   SPINN_CHECK_ARG(l && l->x && l->w && l->y, "linear: x, w and y are required");
   SPINN_CHECK_ARG(l->dtype == SPINN_CUDA_FP16 || l->dtype == SPINN_CUDA_BF16,
                   "linear: element type %d not supported (fp16 or bf16; spinn_cuda_gemm takes fp32)", l->dtype);
-  SPINN_CHECK_ARG(l->m > 0 && l->n > 0 && l->k > 0, "linear: bad sizes %d x %d x %d", l->m, l->n, l->k);
+  SPINN_CHECK_ARG(l->m > 0 && l->n > 0 && l->k > 0 && l->m <= kMaxLength && l->n <= kMaxLength && l->k <= kMaxLength,
+                  "linear: bad sizes %d x %d x %d", l->m, l->n, l->k);
   SPINN_CHECK_ARG(l->x_stride >= l->k && l->w_stride >= l->k && l->y_stride >= l->n &&
                       (!l->residual || l->residual_stride >= l->n),
                   "linear: a row stride is shorter than its row");
@@ -955,6 +956,16 @@ __attribute__((visibility("default"))) int spinn_cuda_linear(const SpinnCudaLine
                   "linear: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
   rc = decode_error_word(dev, &p.err);
   if (rc) return rc;
+  const auto rows = [](const void* q, int count, int width, int64_t stride) {
+    return Rows{q, 2, width, {count, 1, 1}, {stride, 0, 0}};
+  };
+  const Rows y = rows(l->y, l->m, l->n, l->y_stride);
+  SPINN_CHECK_ARG(rows_apart(y, rows(l->x, l->m, l->k, l->x_stride)) && rows_apart(y, rows(l->w, l->n, l->k, l->w_stride)) &&
+                      (!l->bias || rows_apart(y, rows(l->bias, 1, l->n, l->n))),
+                  "linear: y overlaps x, w or bias");
+  SPINN_CHECK_ARG(!l->residual || (l->residual == l->y && (l->m == 1 || l->residual_stride == l->y_stride)) ||
+                      rows_apart(y, rows(l->residual, l->m, l->n, l->residual_stride)),
+                  "linear: y must be the residual itself or apart from it");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return l->dtype == SPINN_CUDA_FP16 ? linear_launch<__half>(p, pl, workspace, sms, st)
                                      : linear_launch<__nv_bfloat16>(p, pl, workspace, sms, st);

@@ -76,6 +76,7 @@ _SIGS = {
     "spinn_cuda_linear": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "spinn_cuda_diag_cache_slot": (ctypes.c_int64, [ctypes.POINTER(ctypes.c_int32)] + [ctypes.c_int] * 4 +
                                    [ctypes.c_int64] * 2),
+    "spinn_cuda_diag_rows": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int64)] * 2),
     "spinn_cuda_diag_attention_share": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int64,
                                                        ctypes.POINTER(ctypes.c_int64)]),
     "spinn_cuda_load": (ctypes.c_void_p, [ctypes.c_char_p]),

@@ -218,6 +218,46 @@ def test_attention_shares_cover_the_work_once():
     assert L.spinn_cuda_diag_attention_share(0, 1, 0, 0, out) == lib.EINVAL
 
 
+def rows(at, width, counts, strides, es=2):
+    counts, strides = (list(counts) + [1] * 3)[:3], (list(strides) + [0] * 3)[:3]
+    return (ctypes.c_int64 * 9)(at, es, width, *counts, *strides)
+
+
+def elements(r):
+    at, es, width, *cs = r
+    out = [at + es * (i * cs[3] + j * cs[4] + k * cs[5] + e) + byte for i in range(cs[0]) for j in range(cs[1])
+           for k in range(cs[2]) for e in range(width) for byte in range(es)]
+    return out, set(out)
+
+
+def test_overlaps_are_found():
+    """No overlap passes, and what decoders do is not refused: slices of one buffer, orders of dimensions."""
+    L = lib.lib()
+    rng = np.random.default_rng(5)
+    seen = [0, 0]
+    for _ in range(4000):
+        a, b = [rows(4096 + 2 * int(rng.integers(-30, 30)), int(rng.integers(1, 6)), rng.integers(1, 4, 2).tolist(),
+                     rng.choice([0, 1, 4, 5, 6, 12, 18, 24], 2).tolist()) for _ in range(2)]
+        (la, sa), (lb, sb) = elements(a), elements(b)
+        got = L.spinn_cuda_diag_rows(a, b)
+        if got & 1:
+            assert len(la) == len(sa), list(a)
+            seen[0] += 1
+        if got & 2:
+            assert not sa & sb, (list(a), list(b))
+            seen[1] += 1
+    assert min(seen) > 400
+    far = rows(1 << 20, 8, (2, 2), (0, 0))
+    for counts, strides in [((3, 8), (64, 8)), ((3, 8), (8, 24)), ((3, 8), (512, 16)), ((1, 1), (0, 0)), ((1, 4), (5, 8))]:
+        assert L.spinn_cuda_diag_rows(rows(0, 8, counts, strides), far) == 3
+    # query, key and value slices of one projection's rows, and y beside them
+    assert L.spinn_cuda_diag_rows(rows(0, 64, (5, 8), (1024, 64)), rows(2 * 512, 64, (5, 4), (1024, 64))) & 2
+    assert not L.spinn_cuda_diag_rows(rows(0, 64, (5, 8), (1024, 64)), rows(2 * 448, 64, (5, 4), (1024, 64))) & 2
+    assert not L.spinn_cuda_diag_rows(rows(0, 8, (2,), (0,)), rows(1 << 20, 8, (1,), (0,))) & 1
+    assert L.spinn_cuda_diag_rows(rows(0, 8, (1,), (0,)), rows(16, 8, (1,), (0,))) == 3
+
+
+
 # ------------------------------------------------------------------ linear
 def linear(**kw):
     f = dict(x=P, w=P, b=0, r=0, y=P, ldx=64, ldw=64, ldr=0, ldy=32, m=4, n=32, k=64, dtype=lib.BF16, act=0)

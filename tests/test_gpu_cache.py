@@ -347,6 +347,56 @@ def test_two_graphs_share_nothing(rt):
         assert torch.equal(y, y2) and torch.equal(wout, w2)
 
 
+def test_outputs_that_overlap_are_refused(rt):
+    """Results whose rows share memory with one another or with what is read: refused before any work."""
+    from spinn_b200.lib import EINVAL, SpinnCudaError
+    c = Paged("bf16", [40, 17], 2, 64, 16, seed=3, room=4)
+    q = torch.randn(2, 4, 64, device="cuda").bfloat16()
+    w = torch.zeros(2, 2, 64, device="cuda")
+
+    def refused(match, fn, *args):
+        with pytest.raises(SpinnCudaError, match=match) as e:
+            fn(*args)
+        assert e.value.code == EINVAL
+
+    attend = lambda q, y, win=None, wout=None: rt.paged_attention(q, c.k, c.v, c.table, c.lens, y, None, win, wout)  # noqa: E731
+    refused("y overlap", attend, q, q)
+    refused("y overlap", attend, q, torch.empty(2, 1, 64, device="cuda").bfloat16().expand(2, 4, 64))
+    refused("weights_out overlap", attend, q, torch.empty_like(q), None, w[:, :1].expand(2, 2, 64))
+    wide = torch.zeros(2, 2, 96, device="cuda")
+    refused("apart from it", attend, q, torch.empty_like(q), wide[..., :64], wide[..., 32:])
+    # query and result side by side in one buffer
+    both = torch.randn(2, 8, 64, device="cuda").bfloat16()
+    y = torch.empty_like(q)
+    attend(both[:, :4], both[:, 4:])
+    attend(both[:, :4].contiguous(), y)
+    rt.stream_sync()
+    assert torch.equal(both[:, 4:], y)
+    one = c.k[:, :, :1].expand(-1, -1, 2, -1)
+    rows = torch.randn(2, 2, 64, device="cuda").bfloat16()
+    refused("pools", rt.cache_append, rows, rows, one, c.v[:, :, :1].expand(-1, -1, 2, -1), c.table, c.lens)
+    refused("pools", rt.cache_append, rows, rows, c.k, c.k, c.table, c.lens)
+    new_lens, kept = torch.empty(2, dtype=torch.int32, device="cuda"), torch.empty(2, 2, 8, dtype=torch.int32, device="cuda")
+    refused("pools", rt.cache_evict, c.k, c.k, c.table, c.lens, w, w, c.table, new_lens, kept, 8)
+    refused("weights_out overlap", rt.cache_evict, c.k, c.v, c.table, c.lens, w, w[:1, :1].clone().expand(2, 2, 64), c.table, new_lens,
+            kept, 8)
+
+
+def test_sync_of_a_capturing_stream_is_refused(rt):
+    """The refusal leaves the capture whole."""
+    from spinn_b200.lib import SpinnCudaError
+    c, q, y, _win, _wout = _attention_case(rt, ("fp16", [100, 7], 4, 2, 64, 16, "nhd", False), seed=9)
+    y2 = torch.zeros_like(y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rt.paged_attention(q, c.k, c.v, c.table, c.lens, y2)
+        with pytest.raises(SpinnCudaError, match="being captured"):
+            rt.stream_sync()
+    graph.replay()
+    rt.stream_sync()
+    assert torch.equal(y, y2)
+
+
 def test_bad_pages_and_lengths_are_reported(rt):
     """A page outside the pool or a length beyond the table is never followed: the operator skips
     it and the next stream_sync raises, once."""

@@ -110,6 +110,25 @@ def test_linear_in_place_of_its_residual(rt):
         assert torch.equal(y, r)
 
 
+@pytest.mark.parametrize("m", [4, 40])
+def test_linear_of_slices_of_one_buffer(rt, m):
+    """x and y as column slices of the same rows; a y that reaches into what is read is refused."""
+    from spinn_b200.lib import EINVAL, SpinnCudaError
+    buf = torch.randn(m, 64 + 48, device="cuda").half()
+    w = torch.randn(48, 64, device="cuda").half()
+    want = torch.empty(m, 48, device="cuda").half()
+    rt.linear(buf[:, :64].clone(), w, want)
+    rt.linear(buf[:, :64], w, buf[:, 64:])
+    rt.stream_sync()
+    assert torch.equal(buf[:, 64:], want)
+    res = torch.randn(m, 96, device="cuda").half()
+    for args in ((buf[:, :64], w, buf[:, 56:104]), (w[:m, :48], torch.randn(48, 48, device="cuda").half(), w[:m, :48]),
+                 (buf[:, :64], w, res[:, :48], None, res[:, 24:72]), (buf[:, :64], w, res[:, :48], res[0, 47:95])):
+        with pytest.raises(SpinnCudaError, match="overlaps|apart") as e:
+            rt.linear(*args)
+        assert e.value.code == EINVAL
+
+
 def test_linear_extreme_activations(rt):
     """Large and infinite pre-activations: the activations' limits, no NaN from inf - inf."""
     eye = torch.eye(16, device="cuda", dtype=torch.bfloat16)
