@@ -134,15 +134,17 @@ __device__ __forceinline__ void mma_rows(float (&c)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Elements k .. k + 7 of a row (zeros past `end`; nothing is read where !row).
+// Elements k .. k + 7 of a row (zeros past `end`; nothing is read where !live).  Operands are read
+// by ordinary loads: a kernel that starts while its predecessor still writes them may not take the
+// read-only path.
 template <bool VEC>
 __device__ __forceinline__ uint4 load8(const uint16_t* row, bool live, int k, int end) {
   uint4 r = make_uint4(0, 0, 0, 0);
   if (!live || k >= end) return r;
-  if (VEC && k + 8 <= end) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  if (VEC && k + 8 <= end) return *reinterpret_cast<const uint4*>(row + k);
   uint32_t h[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) h[i] = k + i < end ? __ldg(row + k + i) : 0;
+  for (int i = 0; i < 8; ++i) h[i] = k + i < end ? row[k + i] : 0;
   r.x = h[0] | h[1] << 16;
   r.y = h[2] | h[3] << 16;
   r.z = h[4] | h[5] << 16;
@@ -237,8 +239,8 @@ __global__ void __launch_bounds__(256) pitch_kernel(const PitchParams p) {
         lo[u] = hi[u] = make_uint4(0, 0, 0, 0);
         if (i < pieces) {
           const uint4* word = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(src + i * 8) & ~uintptr_t(15));
-          lo[u] = __ldg(word);
-          if (shift + min(8, p.k - i * 8) > 8) hi[u] = __ldg(word + 1);
+          lo[u] = *word;
+          if (shift + min(8, p.k - i * 8) > 8) hi[u] = word[1];
         }
       }
 #pragma unroll
@@ -581,8 +583,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
               if (orow + 2 * j < rows)
-                res[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.res) +
-                                                              (long long)(m0 + c + orow + 2 * j) * p.ldr + on));
+                res[j] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.res) +
+                                                         (long long)(m0 + c + orow + 2 * j) * p.ldr + on);
           }
           // the same for rows off alignment, as they are stored below
           const int n0 = (tn * PAIR + side) * 128, width = min(128, p.n - n0);
