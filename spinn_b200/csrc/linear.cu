@@ -1,8 +1,9 @@
 // linear.cu -- y = act(x w^T + bias) + residual in 16-bit types, accumulated in fp32.
 //
-// Two kernels, by the number of rows m of x:
+// Two kernels, by the number of rows m of x and the size of w (see linear_plan):
 //
-// * linear_rows_kernel, m <= 16 (single tokens, small decoding batches): bound by reading w once.
+// * linear_rows_kernel, m <= 16 (single tokens, small decoding batches) with a w that its CTAs
+//   cover in about one wave: bound by reading w once.
 //   No staging: the fragments of mma.sync come straight from global memory, 16 bytes per lane,
 //   with k permuted the same way in both operands so that a lane's 16 contiguous bytes are its
 //   fragment.  Any alignment.
@@ -30,7 +31,7 @@ namespace {
 
 constexpr uint64_t kTimeoutNs = 4000000000ull;  // bounded barrier waits
 constexpr uint64_t kDrainNs = 1000000000ull;
-constexpr int kRowsMax = 16;  // rows of x that linear_rows_kernel takes
+constexpr int kRowsMax = 16;  // most rows of x that linear_rows_kernel takes
 
 struct LinearParams {
   const void* x;
@@ -156,8 +157,10 @@ constexpr int kRowWarps = 8;
 
 // CTA: 16 rows of w, all rows of x (NT blocks of 8); its warps take interleaved 128-element
 // chunks of k and are summed in order through shared memory.
+constexpr int row_ctas(int nt) { return nt == 1 ? 3 : 2; }  // at a time on an SM
+
 template <typename T, int NT, bool VEC>
-__global__ void __launch_bounds__(kRowWarps * 32) linear_rows_kernel(const LinearParams p) {
+__global__ void __launch_bounds__(kRowWarps * 32, row_ctas(NT)) linear_rows_kernel(const LinearParams p) {
   __shared__ float part[kRowWarps][NT * 8][16];
   griddep_launch_dependents();
   griddep_wait();
@@ -769,7 +772,6 @@ bool tma_rows(const void* p, long long ld) { return ((uintptr_t)p & 15) == 0 && 
 
 LinearPlan linear_plan(const LinearParams& p, int sms) {
   LinearPlan pl;
-  if (p.m <= kRowsMax) return pl;
   const size_t pitch = ((size_t)p.k + 7) / 8 * 8 * 2;
   pl.copy_x = !tma_rows(p.x, p.ldx);
   pl.copy_w = !tma_rows(p.w, p.ldw);
@@ -805,6 +807,25 @@ LinearPlan linear_plan(const LinearParams& p, int sms) {
     for (int bn = 32; bn <= 128; bn *= 2) consider(bn, 1, split);
   for (int split = 1; split <= 4; split *= 2) consider(128, 2, split);
   consider(256, 2, 1);
+  if (p.m > kRowsMax) return pl;
+  // The kernel for few rows, or these tiles?  Tiles read w at HBM's bandwidth at best, after 9,500
+  // clocks of start and finish; rows off alignment cost a copy of them first.  The other kernel
+  // takes waves of CTAs through k, 1,024 elements at a time: longer the more of them share an SM,
+  // and some three times as long off alignment.  Fitted to 1, 8 and 16 rows of 28 sizes (us, few-rows
+  // kernel : tiles; 1 x 1024 x 4096 3.0 : 5.6, 8 x 4096 x 1000 4.9 : 5.8, 8 x 4096 x 4096 10.0 : 10.4,
+  // 8 x 4096 x 8192 18.7 : 15.3, 16 x 4096 x 4096 10.7 : 10.6, 16 x 11008 x 4096 22.5 : 19.3, 16 x 4096
+  // x 32000 61.1 : 45.1; off alignment 1 x 1001 x 1000 6.2 : 7.3, 8 x 4095 x 4096 31.1 : 21.9).
+  const double hbm = 5.9e-4;  // clocks for an element read, or for a byte copied
+  const double tiles = std::max(best, 9500.0 + hbm * p.n * p.k) +
+                       (pl.copy_x || pl.copy_w ? 3500.0 + hbm * (double)(pl.x_bytes + pl.w_bytes) : 0.0);
+  const int nt = p.m <= 8 ? 1 : 2;
+  const long long ctas = (p.n + 15) / 16, at_once = (long long)row_ctas(nt) * sms;
+  const double waves = (double)((ctas + at_once - 1) / at_once);
+  const double share = std::min((double)row_ctas(nt), (double)ctas / sms);
+  const double steps = p.k >= 1024 ? p.k / 1024.0 : 0.5 + p.k / 2048.0;
+  double step = (nt == 1 ? 1500.0 : 2200.0) + 1100.0 * share;
+  if (!p.vec) step *= 3.4;
+  if (2600.0 + waves * (1000.0 + steps * step) <= tiles) return LinearPlan();
   return pl;
 }
 
@@ -939,7 +960,12 @@ extern "C" {
 __attribute__((visibility("default"))) size_t spinn_cuda_linear_workspace(const SpinnCudaLinear* l) {
   LinearParams p;
   if (linear_params(l, &p)) return 0;
-  const LinearPlan pl = linear_plan(p, 148);  // the copies do not depend on the SM count
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    dev = -1;
+  }
+  const LinearPlan pl = linear_plan(p, dev < 0 ? 148 : sm_count(dev));
   return pl.x_bytes + pl.w_bytes;
 }
 

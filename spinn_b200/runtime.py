@@ -152,7 +152,7 @@ def linear(x, w, y, bias=None, residual=None, act: str = "none") -> None:
     ``x`` is ``[m, k]``, ``w`` ``[n, k]``, ``y`` and ``residual`` ``[m, n]``, with contiguous rows of any
     stride, ``bias`` ``[n]``; ``act`` is "none", "relu", "silu", "gelu" (by erf) or "gelu_tanh".  ``y``
     may be ``residual`` itself.  Rows of ``x`` and ``w`` that start on 16-byte boundaries are read in
-    place; others are copied first when ``x`` has more than 16 rows."""
+    place; others are copied first where tiles serve better than the kernel for few rows."""
     code = _ACTS.get(act)
     if code is None:
         raise ValueError(f"linear: act must be one of {', '.join(_ACTS)}")

@@ -110,6 +110,24 @@ def test_linear_in_place_of_its_residual(rt):
         assert torch.equal(y, r)
 
 
+@pytest.mark.parametrize("m,k,n,pad", [(1, 8192, 2048, 0), (8, 4096, 8192, 0), (16, 1024, 8200, 0), (16, 8192, 1024, 8),
+                                       (1, 4095, 4100, 0), (12, 3001, 2304, 3), (5, 16000, 33, 0)])
+def test_linear_few_rows_of_large_weights(rt, m, k, n, pad):
+    """Few rows of x with a w that goes to the tiles, aligned or copied first, with its whole epilogue."""
+    dtype = torch.bfloat16
+    x, w, res = rows((m, k), dtype, pad), rows((n, k), dtype, pad, scale=k ** -0.5), rows((m, n), dtype)
+    bias, y = torch.randn(n, device="cuda").to(dtype), torch.full((m + 1, n), 7.0, device="cuda", dtype=dtype)
+    rt.linear(x, w, y[:m], bias, res, "relu")
+    rt.stream_sync()
+    z = x.double() @ w.double().T + bias.double()
+    want = z.relu() + res.double()
+    mass = x.double().abs() @ w.double().abs().T + bias.double().abs()
+    # as above: k 2^-23 of the sum of magnitudes, fp32 adds, one rounding to bf16
+    tol = 2.0 ** -8 * want.abs() + (1 + 2.0 ** -8) * (k * 2.0 ** -23 * mass + 2.0 ** -22 * (z.abs() + want.abs()))
+    assert ((y[:m].double() - want).abs() <= tol).all()
+    assert (y[m] == 7.0).all()
+
+
 @pytest.mark.parametrize("m", [4, 40])
 def test_linear_of_slices_of_one_buffer(rt, m):
     """x and y as column slices of the same rows; a y that reaches into what is read is refused."""
