@@ -2,7 +2,7 @@
 //
 // Two kernels, by the number of rows m of x and the size of w (see linear_plan):
 //
-// * linear_rows_kernel, m <= 16 (single tokens, small decoding batches) with a w that its CTAs
+// * linear_rows_kernel, m <= 32 (single tokens, small decoding batches) with a w that its CTAs
 //   cover in about one wave: bound by reading w once.
 //   No staging: the fragments of mma.sync come straight from global memory, 16 bytes per lane,
 //   with k permuted the same way in both operands so that a lane's 16 contiguous bytes are its
@@ -31,7 +31,7 @@ namespace {
 
 constexpr uint64_t kTimeoutNs = 4000000000ull;  // bounded barrier waits
 constexpr uint64_t kDrainNs = 1000000000ull;
-constexpr int kRowsMax = 16;  // most rows of x that linear_rows_kernel takes
+constexpr int kRowsMax = 32;  // most rows of x that linear_rows_kernel takes
 
 struct LinearParams {
   const void* x;
@@ -155,10 +155,11 @@ __device__ __forceinline__ uint4 load8(const uint16_t* row, bool live, int k, in
 
 constexpr int kRowWarps = 8;
 
-// CTA: 16 rows of w, all rows of x (NT blocks of 8); its warps take interleaved 128-element
-// chunks of k and are summed in order through shared memory.
 constexpr int row_ctas(int nt) { return nt == 1 ? 3 : 2; }  // at a time on an SM
 
+// CTA: 16 rows of w, all rows of x (NT blocks of 8); its warps take interleaved chunks of k and are
+// summed in order through shared memory.  Asking for the next chunk before this one is used gained
+// 13% on 1 x 4096 x 4096 and cost more elsewhere (8 x 4096 x 11008 19.6 -> 21.7 us: fewer CTAs at a time).
 template <typename T, int NT, bool VEC>
 __global__ void __launch_bounds__(kRowWarps * 32, row_ctas(NT)) linear_rows_kernel(const LinearParams p) {
   __shared__ float part[kRowWarps][NT * 8][16];
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, row_ctas(NT)) linear_rows_kern
   float acc[NT][4];
 #pragma unroll
   for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.0f;
-  constexpr int U = 4;  // 32-element steps in flight
+  constexpr int U = NT == 4 ? 2 : 4;  // 32-element steps in flight: what the registers hold
   for (int k0 = warp * 32 * U; k0 < p.k; k0 += kRowWarps * 32 * U) {
     uint4 a[U], b[U], x[U][NT];
 #pragma unroll
@@ -807,23 +808,24 @@ LinearPlan linear_plan(const LinearParams& p, int sms) {
     for (int bn = 32; bn <= 128; bn *= 2) consider(bn, 1, split);
   for (int split = 1; split <= 4; split *= 2) consider(128, 2, split);
   consider(256, 2, 1);
-  if (p.m > kRowsMax) return pl;
+  if (p.m > (p.vec ? kRowsMax : 16)) return pl;
   // The kernel for few rows, or these tiles?  Tiles read w at HBM's bandwidth at best, after 9,500
   // clocks of start and finish; rows off alignment cost a copy of them first.  The other kernel
   // takes waves of CTAs through k, 1,024 elements at a time: longer the more of them share an SM,
-  // and some three times as long off alignment.  Fitted to 1, 8 and 16 rows of 28 sizes (us, few-rows
-  // kernel : tiles; 1 x 1024 x 4096 3.0 : 5.6, 8 x 4096 x 1000 4.9 : 5.8, 8 x 4096 x 4096 10.0 : 10.4,
-  // 8 x 4096 x 8192 18.7 : 15.3, 16 x 4096 x 4096 10.7 : 10.6, 16 x 11008 x 4096 22.5 : 19.3, 16 x 4096
-  // x 32000 61.1 : 45.1; off alignment 1 x 1001 x 1000 6.2 : 7.3, 8 x 4095 x 4096 31.1 : 21.9).
+  // and some three times as long off alignment.  Fitted to 1, 8, 16 and 32 rows of 28 sizes (us,
+  // few-rows kernel : tiles; 1 x 1024 x 4096 3.0 : 5.6, 8 x 4096 x 1000 4.9 : 5.8, 8 x 4096 x 4096
+  // 10.0 : 10.4, 8 x 4096 x 8192 18.7 : 15.3, 16 x 4096 x 4096 10.7 : 10.6, 16 x 11008 x 4096 22.5 :
+  // 19.3, 16 x 4096 x 32000 61.1 : 45.1, 32 x 1024 x 1024 3.7 : 5.0, 32 x 2048 x 2048 6.6 : 5.9; off
+  // alignment 1 x 1001 x 1000 6.2 : 7.3, 8 x 4095 x 4096 31.1 : 21.9; past 16 rows 10 : 7.5).
   const double hbm = 5.9e-4;  // clocks for an element read, or for a byte copied
   const double tiles = std::max(best, 9500.0 + hbm * p.n * p.k) +
                        (pl.copy_x || pl.copy_w ? 3500.0 + hbm * (double)(pl.x_bytes + pl.w_bytes) : 0.0);
-  const int nt = p.m <= 8 ? 1 : 2;
+  const int nt = p.m <= 8 ? 1 : p.m <= 16 ? 2 : 4;
   const long long ctas = (p.n + 15) / 16, at_once = (long long)row_ctas(nt) * sms;
   const double waves = (double)((ctas + at_once - 1) / at_once);
   const double share = std::min((double)row_ctas(nt), (double)ctas / sms);
   const double steps = p.k >= 1024 ? p.k / 1024.0 : 0.5 + p.k / 2048.0;
-  double step = (nt == 1 ? 1500.0 : 2200.0) + 1100.0 * share;
+  double step = (nt == 1 ? 1500.0 : nt == 2 ? 2200.0 : 3600.0) + 1100.0 * share;
   if (!p.vec) step *= 3.4;
   if (2600.0 + waves * (1000.0 + steps * step) <= tiles) return LinearPlan();
   return pl;
@@ -875,6 +877,7 @@ int linear_launch(const LinearParams& p, const LinearPlan& pl, void* ws, int sms
     if (p.m <= 8)
       return p.vec ? launch_dependent(linear_rows_kernel<T, 1, true>, grid, threads, 0, st, p)
                    : launch_dependent(linear_rows_kernel<T, 1, false>, grid, threads, 0, st, p);
+    if (p.m > 16) return launch_dependent(linear_rows_kernel<T, 4, true>, grid, threads, 0, st, p);
     return p.vec ? launch_dependent(linear_rows_kernel<T, 2, true>, grid, threads, 0, st, p)
                  : launch_dependent(linear_rows_kernel<T, 2, false>, grid, threads, 0, st, p);
   }

@@ -111,9 +111,10 @@ def test_linear_in_place_of_its_residual(rt):
 
 
 @pytest.mark.parametrize("m,k,n,pad", [(1, 8192, 2048, 0), (8, 4096, 8192, 0), (16, 1024, 8200, 0), (16, 8192, 1024, 8),
-                                       (1, 4095, 4100, 0), (12, 3001, 2304, 3), (5, 16000, 33, 0)])
+                                       (1, 4095, 4100, 0), (12, 3001, 2304, 3), (5, 16000, 33, 0), (17, 1000, 1031, 0),
+                                       (32, 520, 4096, 8), (25, 1024, 513, 0)])
 def test_linear_few_rows_of_large_weights(rt, m, k, n, pad):
-    """Few rows of x with a w that goes to the tiles, aligned or copied first, with its whole epilogue."""
+    """Few rows of x on both sides of the choice of a kernel, aligned or copied first, with the whole epilogue."""
     dtype = torch.bfloat16
     x, w, res = rows((m, k), dtype, pad), rows((n, k), dtype, pad, scale=k ** -0.5), rows((m, n), dtype)
     bias, y = torch.randn(n, device="cuda").to(dtype), torch.full((m + 1, n), 7.0, device="cuda", dtype=dtype)
