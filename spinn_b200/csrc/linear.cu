@@ -346,6 +346,17 @@ union Pair {
   __device__ Pair() {}
 };
 
+template <typename T>
+__device__ __forceinline__ uint32_t round_pair(float a, float b) {  // a in the low half
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
 constexpr int kTileThreads = 384;  // producer, MMA, TMEM and a spare warp, eight epilogue warps
 
 // BN: rows of x of a tile.  PAIR 2: a CTA pair works on 256 rows of w with one cta_group::2 MMA
@@ -708,19 +719,29 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const bool one = n < p.n, two = n + 1 < p.n;
     const float bias0 = p.bias && one ? to_float(static_cast<const T*>(p.bias)[n]) : 0.0f;
     const float bias1 = p.bias && two ? to_float(static_cast<const T*>(p.bias)[n + 1]) : 0.0f;
-    const bool words = ((uintptr_t)p.y & 3) == 0 && (p.ldy & 1) == 0;
+    const bool words = two && ((uintptr_t)p.y & 3) == 0 && (p.ldy & 1) == 0;  // n is even
+    const bool res_words = two && ((uintptr_t)p.res & 3) == 0 && (p.ldr & 1) == 0;
     const float4* sums = reinterpret_cast<const float4*>(part);
     const int plane = BN / 4 / (int)splits * 128;
     bool joined = false;
     for (int g = threadIdx.x >> 6; g < mine || !joined; g += kTileThreads / 64) {
       const int row = (g * (int)splits + (int)rank) * 4, m = tm * BN + row;
-      float res[4][2];
+      float res[4][2] = {};
+      if (p.res && one && g < mine) {
+        const T* src = static_cast<const T*>(p.res) + (long long)m * p.ldr + n;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bool live = p.res && g < mine && row + e < rows;
-        const T* src = static_cast<const T*>(p.res) + (live ? (long long)(m + e) * p.ldr + n : 0);
-        res[e][0] = live && one ? to_float(src[0]) : 0.0f;
-        res[e][1] = live && two ? to_float(src[1]) : 0.0f;
+        for (int e = 0; e < 4; ++e, src += p.ldr) {
+          if (row + e >= rows) continue;
+          if (res_words) {
+            Pair<T> x;
+            x.u = *reinterpret_cast<const uint32_t*>(src);
+            res[e][0] = to_float(x.t[0]);
+            res[e][1] = to_float(x.t[1]);
+          } else {
+            res[e][0] = to_float(src[0]);
+            if (two) res[e][1] = to_float(src[1]);
+          }
+        }
       }
       if (!joined) {
         if (PAIR == 1 && warp < 4) cluster_wait();
@@ -747,18 +768,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] += e & 1 ? bias1 : bias0;
       activate(v, p.act);
+      if (p.res)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 8; ++e) v[e] += res[e >> 1][e & 1];
+      T* dst = static_cast<T*>(p.y) + (long long)m * p.ldy + n;
+#pragma unroll
+      for (int e = 0; e < 4; ++e, dst += p.ldy) {
         if (row + e >= rows) continue;
-        T* dst = static_cast<T*>(p.y) + (long long)(m + e) * p.ldy + n;
-        Pair<T> x;
-        x.t[0] = round_to<T>(p.res ? v[2 * e] + res[e][0] : v[2 * e]);
-        x.t[1] = round_to<T>(p.res ? v[2 * e + 1] + res[e][1] : v[2 * e + 1]);
-        if (words && two) {
-          *reinterpret_cast<uint32_t*>(dst) = x.u;
+        if (words) {
+          *reinterpret_cast<uint32_t*>(dst) = round_pair<T>(v[2 * e], v[2 * e + 1]);
         } else {
-          dst[0] = x.t[0];
-          if (two) dst[1] = x.t[1];
+          dst[0] = round_to<T>(v[2 * e]);
+          if (two) dst[1] = round_to<T>(v[2 * e + 1]);
         }
       }
     }
