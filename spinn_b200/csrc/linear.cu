@@ -812,13 +812,13 @@ LinearPlan linear_plan(const LinearParams& p, int sms) {
   pl.copy_w = !tma_rows(p.w, p.ldw);
   pl.x_bytes = pl.copy_x ? (pitch * p.m + 255) / 256 * 256 : 0;
   pl.w_bytes = pl.copy_w ? (pitch * p.n + 255) / 256 * 256 : 0;
-  // Shape by estimated clocks, fitted to a sweep of every shape over 30 sizes (device time in a
-  // captured queue).  A stage of 128 k takes as long as its operands need to pass through shared
-  // memory twice (written by TMA, read by the MMA at 128 bytes a clock): about 870 clocks for a
-  // single CTA whatever its width up to 128, 950 and 1,150 for the pairs (700 for split ones, which run
-  // alone on memory-bound problems).  Around the stages lie
-  // the launch and first loads (2,600; 900 more for a cluster), and the last tile's epilogue.
-  // Splitting k pays when there are few tiles: it adds the exchange of the partial sums.
+  // Shape by estimated clocks, fitted to a sweep of every shape over 41 sizes (device time in a
+  // captured queue; what it picks takes 0.5% longer than the best, geometric mean).  A stage of 128
+  // k takes 600, 650 and 870 clocks on a single CTA of 32, 64 and 128 columns -- the issue of its
+  // eight MMAs and the barriers around them, then the operands' way into shared memory -- and 800
+  // and 1,200 on pairs (650 split).  Around the stages lie the launch and first loads (2,600; 900
+  // more for a cluster), and the last tile's epilogue.  Splitting k pays when there are few tiles:
+  // it adds the exchange of the partial sums.
   const int kb = (p.k + 127) / 128;
   double best = 0;
   auto consider = [&](int bn, int pair, int split) {
@@ -827,10 +827,11 @@ LinearPlan linear_plan(const LinearParams& p, int sms) {
     if (split > 1 && (waves > 1 || kb < 2 * split)) return;
     // clusters that the GPCs of 148 SMs hold at once
     if (split > 1 && (split * pair == 8 ? tiles > 15 : split * pair == 4 && tiles > 34)) return;
-    const double stage = pair == 1 ? 870.0 : bn == 256 ? 1150.0 : split > 1 ? 700.0 : 950.0;
+    const double stage = pair == 1 ? (bn == 32 ? 600.0 : bn == 64 ? 650.0 : 870.0)
+                                   : bn == 256 ? 1200.0 : split > 1 ? 650.0 : 800.0;
     double clocks = 2600.0 + (pair * split > 1 ? 900.0 : 0.0) + (double)waves * ((kb + split - 1) / split) * stage;
     clocks += bn * 30.0 + 300.0;
-    if (split > 1) clocks += 1100.0 + bn * 26.0 / split + (pair == 2 ? 1700.0 : 0.0);
+    if (split > 1) clocks += 1100.0 + bn * 26.0 / split + (pair == 2 ? 1000.0 : 0.0);
     if (pl.bn == 0 || clocks < best) {
       pl.bn = bn;
       pl.pair = pair;
