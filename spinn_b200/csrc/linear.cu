@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
       __syncwarp();
     }
-    if (warp_abort(abort_flag) && issued && lane == 0) {
+    if (warp_abort(abort_flag) && issued && elect_one()) {  // the lane that issued
       volatile int dummy = 0;
       if constexpr (PAIR == 2)
         umma_commit_pair(mapa_shared(smem_u32(drain), leader));
