@@ -6,7 +6,7 @@
 //   cover in about one wave: bound by reading w once.
 //   No staging: the fragments of mma.sync come straight from global memory, 16 bytes per lane,
 //   with k permuted the same way in both operands so that a lane's 16 contiguous bytes are its
-//   fragment.  Any alignment.
+//   fragment.  Any alignment up to 16 rows, aligned rows past them.
 //
 // * linear_tile_kernel: tcgen05 with TMA-fed swizzled stages.  The rows of w are the MMA's rows
 //   (TMEM lanes) and the rows of x its columns, i.e. it computes y^T tiles: a warp that drains
