@@ -204,7 +204,9 @@ int spinn_cuda_cache_append(const SpinnCudaCache *cache, const SpinnCudaPageTabl
  *   y[s][h] = sum_t p[s][h][t] v[s][h / group][t],  p = softmax over t < lens[s] of
  *   scale * q[s][h] . k[s][h / group][t],  group = q_heads / kv_heads.
  * q and y are [seqs][q_heads][head_dim] of the cache's type (strides in elements).  A sequence
- * of length 0 gets zeros.  Sums and probabilities are held in fp32 and y is rounded once.
+ * of length 0 gets zeros.  Sums are held in fp32 and y is rounded once; over 16-bit caches a probability
+ * enters the product with v as two 16-bit parts, off by at most 2^-17 of itself (bf16) or of the largest
+ * of 16 tokens around it (fp16).
  * weights_out, when not NULL ([seqs][kv_heads][>= lens[s]] fp32, group <= 16, weights_capacity
  * entries per row): weights_out[s][j][t] = weights_in[s][j][t] + the sum of p[s][h][t] over the
  * heads h of group j, for t < lens[s]; entries beyond are left as they were.  weights_in NULL
