@@ -84,6 +84,12 @@ int spinn_cuda_selftest_wait_expiry(uint64_t timeout_ns);
  * expected result, the context stays usable. */
 int spinn_cuda_selftest_flag_wait_expiry(uint64_t timeout_ns);
 
+/* The same for the wait of four warps that go on together or not at all (the linear layer's
+ * epilogue): a barrier completes after arrive_ns (at most 100 ms), the first warp gives up after
+ * limit_ns (at most 1 s).  Returns the warps that went on, bit by bit: 15 or 0; on the current device and
+ * its default stream. */
+int spinn_cuda_selftest_group_wait(uint64_t arrive_ns, uint64_t limit_ns);
+
 /* Releases the calling thread's session (stream, scratch, cached weights). */
 void spinn_cuda_shutdown(void);
 

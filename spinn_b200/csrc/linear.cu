@@ -332,6 +332,23 @@ __device__ __forceinline__ bool warp_abort(volatile int* abort) { return __any_s
 __device__ __forceinline__ void group_sync(int group) {
   asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory");
 }
+// Waits for `bar` in the four warps of one group, which go on together or give up together: by itself
+// a warp may see another's abort just before the barrier completes, and leave its neighbours in the
+// group_sync that follows.  The vote costs a barrier per tile.
+__device__ __forceinline__ bool group_wait(uint64_t* bar, uint32_t parity, volatile int* abort, uint64_t timeout_ns,
+                                           int group) {
+  const uint32_t mine = __all_sync(0xffffffffu, mbar_wait_backoff(bar, parity, abort, timeout_ns));
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, %2, 128, p;\n\t"
+      "selp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(mine), "r"(group + 1)
+      : "memory");
+  return all != 0;
+}
 template <typename T>
 union Pack {
   uint4 u;
@@ -581,7 +598,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const int m0 = tm * BN;
       const float bias = !SPL && p.bias && n < p.n ? to_float(static_cast<const T*>(p.bias)[n]) : 0.0f;
       const int b = it % NACC;
-      const bool ok = __all_sync(0xffffffffu, mbar_wait_backoff(&tfull[b], (it / NACC) & 1, abort_flag, kTimeoutNs));
+      bool ok;
+      if constexpr (SPL)  // no barrier of the group follows: a warp that gives up goes to the cluster's like the others
+        ok = __all_sync(0xffffffffu, mbar_wait_backoff(&tfull[b], 0, abort_flag, kTimeoutNs));
+      else
+        ok = group_wait(&tfull[b], (it / NACC) & 1, abort_flag, kTimeoutNs, half);
       if (!ok) break;
       tc_fence_after();
       for (int c = half * CW; c < BN && m0 + c < p.m; c += 2 * CW) {
@@ -796,6 +817,35 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
 }
 
+// Four warps of a group wait for a barrier that a fifth completes after `arrive_ns`; the first gives up
+// after `limit_ns`, by an abort flag of its own.  Bit w of the result: warp w goes on.
+__device__ unsigned g_group_wait_verdict;
+__global__ void __launch_bounds__(160) group_wait_selftest_kernel(uint64_t arrive_ns, uint64_t limit_ns) {
+  __shared__ uint64_t bar;
+  __shared__ int abort_flag[2];
+  __shared__ unsigned verdict;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar, 1);
+    fence_mbar_init();
+    abort_flag[0] = abort_flag[1] = 0;
+    verdict = 0;
+  }
+  __syncthreads();
+  if (warp == 4) {
+    if (lane == 0) {
+      const uint64_t t0 = globaltimer_ns();
+      while (globaltimer_ns() - t0 < arrive_ns) __nanosleep(1000);
+      mbar_arrive(&bar);
+    }
+  } else {
+    const bool on = group_wait(&bar, 0, &abort_flag[warp != 0], warp ? kTimeoutNs : limit_ns, 0);
+    if (on && lane == 0) atomicOr(&verdict, 1u << warp);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) g_group_wait_verdict = verdict;
+}
+
 // ------------------------------------------------------------------ host
 struct LinearPlan {
   int bn = 0, pair = 1, split = 1;  // bn 0: linear_rows_kernel
@@ -1005,6 +1055,16 @@ __attribute__((visibility("default"))) size_t spinn_cuda_linear_workspace(const 
   }
   const LinearPlan pl = linear_plan(p, dev < 0 ? 148 : sm_count(dev));
   return pl.x_bytes + pl.w_bytes;
+}
+
+__attribute__((visibility("default"))) int spinn_cuda_selftest_group_wait(uint64_t arrive_ns, uint64_t limit_ns) {
+  SPINN_CHECK_ARG(arrive_ns <= 100000000 && limit_ns > 0 && limit_ns <= 1000000000,
+                  "selftest_group_wait: at most 100 ms to the arrival and a limit of at most 1 s");
+  group_wait_selftest_kernel<<<1, 160>>>(arrive_ns, limit_ns);
+  SPINN_CUDA_TRY(cudaGetLastError());
+  unsigned verdict = 0;
+  SPINN_CUDA_TRY(cudaMemcpyFromSymbol(&verdict, g_group_wait_verdict, sizeof(verdict)));
+  return (int)verdict;
 }
 
 __attribute__((visibility("default"))) int spinn_cuda_linear(const SpinnCudaLinear* l, void* workspace,
