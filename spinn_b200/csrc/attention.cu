@@ -128,5 +128,20 @@ __attribute__((visibility("default"))) int spinn_cuda_paged_attention(const Spin
                                            : attention_launch_fp32(p, pl, st);
 }
 
+__attribute__((visibility("default"))) int spinn_cuda_diag_attention_ring(const int32_t* ops, int count, int32_t* out) {
+  SPINN_CHECK_ARG(ops && out && count >= 0, "diag_attention_ring: invalid arguments");
+  CopyRing r;
+  for (int i = 0; i < count; ++i) {
+    const int s = ops[i] & 15;
+    SPINN_CHECK_ARG((ops[i] >> 4) >= 0 && (ops[i] >> 4) <= 2, "diag_attention_ring: operation %d", ops[i]);
+    const bool armed = ops[i] >> 4 == 0 && r.arm(s);
+    if (ops[i] >> 4) r.waited(s, ops[i] >> 4 == 1);
+    out[3 * i] = armed;
+    out[3 * i + 1] = (int32_t)r.parity;
+    out[3 * i + 2] = (int32_t)r.flight;
+  }
+  return 0;
+}
+
 }  // extern "C"
 }  // namespace spinn

@@ -388,6 +388,7 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
   } else {
     off = row_offset(ahead);
   }
+  CopyRing stages;
   auto issue = [&](int i, int stage) {  // tile i of this share
     uint8_t* kdst = ring + stage * C::STAGE;
     uint8_t* vdst = kdst + C::HALF;
@@ -398,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
       }
       const int page = __shfl_sync(0xffffffffu, now.page, i & 31), tok = __shfl_sync(0xffffffffu, now.tok, i & 31);
       const int head = __shfl_sync(0xffffffffu, now.head, i & 31);
-      if (page == -1) return;  // all of the rows are past the end: the tile is skipped
+      if (page == -1 || !stages.arm(stage)) return;  // all of the rows are past the end: the tile is skipped
       if (page < 0) {
         for (int j = lane; j < 2 * C::HALF / 16; j += 32) reinterpret_cast<uint4*>(kdst)[j] = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
@@ -456,7 +457,6 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
     }
     cp_async_commit();
   }
-  uint32_t phases = 0;  // bit s: parity of the next wait for stage s
 
   // ---- running state of this warp
   uint32_t koff[4], voff[4];  // ldmatrix addresses of the four 16-element steps of a sub-tile
@@ -511,10 +511,9 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
     if (left <= 0) return;
     uint8_t* tile = ring + stage * C::STAGE;
     if (mode == kCopyTma) {
-      if (!mbar_wait(&full[stage], phases >> stage & 1, abort_flag, kTimeoutNs)) {
-        if (lane == 0) atomicOr(p.c.err, kWaitExpired);
-      }
-      phases ^= 1u << stage;
+      const bool landed = mbar_wait(&full[stage], stages.parity_of(stage), abort_flag, kTimeoutNs);
+      if (!landed && lane == 0) atomicOr(p.c.err, kWaitExpired);
+      stages.waited(stage, landed);
       if (left < RW) {
         // what lies behind the end of the cache may be anything, and 0 * NaN is NaN
         if constexpr (C::k16) {
@@ -914,9 +913,11 @@ __global__ void __launch_bounds__(kThreads, Tile<T, DPAD, GB>::CTAS) attention_k
     if (i + 1 < count) walk_next<TK>(p, cur);
   }
   // after an expired wait: copies in flight land before the shared memory goes away
-  if (*abort_flag && mode == kCopyTma) {
-    volatile int dummy = 0;
-    for (int i = 0; i < NS; ++i) mbar_wait(&full[i], phases >> i & 1, &dummy, kDrainNs);
+  if (stages.flight) {
+    for (int i = 0; i < NS; ++i) {
+      volatile int dummy = 0;
+      if (stages.flight >> i & 1) mbar_wait(&full[i], stages.parity_of(i), &dummy, kDrainNs);
+    }
   }
 }
 

@@ -22,6 +22,25 @@ struct Segment {
   int w0, w1;
 };
 
+// Bookkeeping of a warp's ring of stages that TMA fills.  Once a wait has expired nothing is armed any
+// more: a stage whose copy is still in flight may not be armed again, and it is that copy's phase
+// that has to end before the shared memory is given up.
+struct CopyRing {
+  unsigned parity = 0;  // bit s: of the next wait for stage s
+  unsigned flight = 0;  // bit s: armed, not yet seen to land
+  bool expired = false;
+  __host__ __device__ bool arm(int s) {
+    if (!expired) flight |= 1u << s;
+    return !expired;
+  }
+  __host__ __device__ unsigned parity_of(int s) const { return parity >> s & 1; }
+  __host__ __device__ void waited(int s, bool landed) {
+    parity ^= (unsigned)landed << s;
+    flight &= ~((unsigned)landed << s);
+    expired |= !landed;
+  }
+};
+
 enum AttnCopy { kCopyElements = 0, kCopyVec = 1, kCopyTma = 2 };
 
 struct AttnParams {
