@@ -292,6 +292,10 @@ int spinn_cuda_diag_rows(const int64_t *a, const int64_t *b);
 /* Diagnostics (host only): attention's split of `units` tiles over `workers`: out3 = {first unit
  * of `worker`, its end, the worker that owns `unit`}. */
 int spinn_cuda_diag_attention_share(int64_t units, int workers, int worker, int64_t unit, int64_t *out3);
+/* Diagnostics (host only): the kernel that a linear layer takes on `sms` SMs: out5 = {rows of x per tile
+ * (0: the kernel for few rows), CTAs of a pair, ways in which k is split, whether x and w are copied
+ * first}. */
+int spinn_cuda_diag_linear_plan(const SpinnCudaLinear *l, int sms, int *out5);
 /* Diagnostics (host only): attention's bookkeeping of copies in flight.  ops[i] is a stage (0 .. 15), plus
  * 16 for a wait that saw its copy land, 32 for one that expired, else arming it.  Three numbers after
  * each: whether it was armed, the parities of the next waits, the stages in flight (bit by bit). */

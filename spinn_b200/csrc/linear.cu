@@ -1067,6 +1067,20 @@ __attribute__((visibility("default"))) int spinn_cuda_selftest_group_wait(uint64
   return (int)verdict;
 }
 
+__attribute__((visibility("default"))) int spinn_cuda_diag_linear_plan(const SpinnCudaLinear* l, int sms, int* out5) {
+  LinearParams p;
+  const int rc = linear_params(l, &p);
+  if (rc) return rc;
+  SPINN_CHECK_ARG(sms > 0 && out5, "diag_linear_plan: invalid arguments");
+  const LinearPlan pl = linear_plan(p, sms);
+  out5[0] = pl.bn;
+  out5[1] = pl.pair;
+  out5[2] = pl.split;
+  out5[3] = pl.copy_x;
+  out5[4] = pl.copy_w;
+  return 0;
+}
+
 __attribute__((visibility("default"))) int spinn_cuda_linear(const SpinnCudaLinear* l, void* workspace,
                                                              size_t workspace_bytes, void* stream) {
   LinearParams p;

@@ -79,6 +79,7 @@ _SIGS = {
     "spinn_cuda_diag_rows": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int64)] * 2),
     "spinn_cuda_diag_attention_share": (ctypes.c_int, [ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int64,
                                                        ctypes.POINTER(ctypes.c_int64)]),
+    "spinn_cuda_diag_linear_plan": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_int, ctypes.POINTER(ctypes.c_int)]),
     "spinn_cuda_diag_attention_ring": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int32), ctypes.c_int,
                                                       ctypes.POINTER(ctypes.c_int32)]),
     "spinn_cuda_load": (ctypes.c_void_p, [ctypes.c_char_p]),
