@@ -156,7 +156,10 @@ int spinn_cuda_conv2d_noalloc(const float *x, const float *w, const float *bias,
  * calls may be captured into CUDA graphs.  A call that needs a workspace takes it from the
  * caller (the _workspace function gives its size, 16-byte aligned, contents irrelevant before
  * and after); two calls that may overlap on the GPU need two workspaces.  What a call writes has
- * rows apart from one another and from what it reads, but where an operator says otherwise.  Sizes
+ * rows apart from one another and from what it reads, but where an operator says otherwise: operands
+ * of a call that overlap are refused (so are those that interleave with strides which do not tell
+ * them apart), but which rows of a pool a call reads and writes only its page numbers say, and
+ * keeping those apart is the caller's part.  Sizes
  * and lengths are at most 2^31 - 65536.  Arguments are checked before any work is queued
  * (SPINN_CUDA_EINVAL).  What only the device can see -- a page number
  * outside the pool, a length beyond the table -- is skipped by the kernel without touching

@@ -94,15 +94,6 @@ __attribute__((visibility("default"))) int spinn_cuda_paged_attention(const Spin
   AttnParams p;
   int rc = attention_params(cache, table, a, &p);
   if (rc) return rc;
-  int dev;
-  rc = check_stream_device("paged_attention", stream, &dev);
-  if (rc) return rc;
-  rc = decode_error_word(dev, &p.c.err);
-  if (rc) return rc;
-  const AttnPlan pl = attention_plan(p, cache->dtype, sm_count(dev));
-  const size_t need = pl.part + pl.ml + pl.pieces + pl.segs + pl.logits;
-  SPINN_CHECK_ARG(!need || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
-                  "paged_attention: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
   const int es = dtype_bytes(cache->dtype);
   const Rows q = {a->q, es, cache->head_dim, {table->seqs, a->q_heads, 1}, {a->q_seq_stride, a->q_head_stride, 0}};
   const Rows y = {a->y, es, cache->head_dim, {table->seqs, a->q_heads, 1}, {a->y_seq_stride, a->y_head_stride, 0}};
@@ -113,9 +104,20 @@ __attribute__((visibility("default"))) int spinn_cuda_paged_attention(const Spin
     const Rows win = {a->weights_in, 4, a->weights_capacity, {table->seqs, cache->kv_heads, 1},
                       {a->win_seq_stride, a->win_head_stride, 0}};
     SPINN_CHECK_ARG(rows_distinct(wout), "paged_attention: rows of weights_out overlap");
+    SPINN_CHECK_ARG(rows_apart(wout, q) && rows_apart(wout, y) && (!a->weights_in || rows_apart(win, y)),
+                    "paged_attention: weights overlap y, or weights_out q");
     SPINN_CHECK_ARG(!a->weights_in || a->weights_in == a->weights_out || rows_apart(wout, win),
                     "paged_attention: weights_out must be weights_in itself or apart from it");
   }
+  int dev;
+  rc = check_stream_device("paged_attention", stream, &dev);
+  if (rc) return rc;
+  rc = decode_error_word(dev, &p.c.err);
+  if (rc) return rc;
+  const AttnPlan pl = attention_plan(p, cache->dtype, sm_count(dev));
+  const size_t need = pl.part + pl.ml + pl.pieces + pl.segs + pl.logits;
+  SPINN_CHECK_ARG(!need || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0),
+                  "paged_attention: workspace of %zu bytes (16-byte aligned) needed, %zu given", need, workspace_bytes);
   char* ws = static_cast<char*>(workspace);
   p.part = reinterpret_cast<float*>(ws);
   p.ml = reinterpret_cast<float*>(ws + pl.part);

@@ -91,28 +91,46 @@ bool cache_vec16(const CacheView& v, int bytes) {
 
 namespace {
 
-// Extents of nested rows in bytes: of all of them, of one step of the outermost dimension, and
-// that dimension's stride (0: a single row).
+// What rows cover in bytes, and whether their dimensions nest.
 struct Extent {
-  long long all, inner, stride;
+  long long all;
   bool nested;
 };
 
 Extent extent(const Rows& r) {
   int order[3] = {0, 1, 2};
   std::sort(order, order + 3, [&](int a, int b) { return r.stride[a] < r.stride[b]; });
-  Extent e = {r.width * r.bytes, r.width * r.bytes, 0, true};
+  Extent e = {r.width * r.bytes, true};
   for (int i : order) {
     if (r.count[i] <= 1) continue;
-    e.stride = r.stride[i] * r.bytes;
-    e.inner = e.all;
-    e.nested &= e.stride >= e.all;
-    e.all += (r.count[i] - 1) * e.stride;
+    const long long stride = r.stride[i] * r.bytes;
+    e.nested &= stride >= e.all;
+    e.all += (r.count[i] - 1) * stride;
   }
   return e;
 }
 
 }  // namespace
+
+// A dimension of two operands: its stride in bytes, the steps of each, and what each covers below it.
+struct Level {
+  long long stride, na, nb, ea, eb;
+};
+
+// Whether b, d bytes behind a, meets no element of it: at each stride only the few relative steps at which
+// what lies below may meet are followed.  More than a few (one operand's rows are longer than the
+// other's stride) counts as meeting.
+bool levels_apart(const Level* l, int levels, long long d, long long wa, long long wb) {
+  if (!levels) return d >= wa || -d >= wb;
+  const Level& v = l[levels - 1];
+  const auto floor_div = [](long long x, long long y) { return x / y - (x % y < 0); };
+  const long long lo = std::max(floor_div(-v.eb - d, v.stride) + 1, -(v.na - 1));
+  const long long hi = std::min(floor_div(v.ea - 1 - d, v.stride), v.nb - 1);
+  if (hi - lo > 3) return false;
+  for (long long k = lo; k <= hi; ++k)
+    if (!levels_apart(l, levels - 1, d + k * v.stride, wa, wb)) return false;
+  return true;
+}
 
 bool rows_distinct(const Rows& r) { return extent(r).nested; }
 
@@ -120,10 +138,30 @@ bool rows_apart(const Rows& a, const Rows& b) {
   const Extent x = extent(a), y = extent(b);
   const long long d = (long long)((uintptr_t)b.p - (uintptr_t)a.p);
   if (d >= x.all || -d >= y.all) return true;
-  const long long s = x.stride ? x.stride : y.stride;
-  if (!s || !x.nested || !y.nested || (x.stride && y.stride && x.stride != y.stride)) return false;
-  const long long at = (d % s + s) % s;
-  return at >= x.inner && at + y.inner <= s;
+  if (!x.nested || !y.nested) return false;
+  Level l[6];
+  int n = 0;
+  const auto add = [&](const Rows& r, bool first) {
+    for (int i = 0; i < 3; ++i) {
+      if (r.count[i] <= 1) continue;
+      const long long s = r.stride[i] * r.bytes;
+      int j = 0;
+      while (j < n && l[j].stride != s) ++j;
+      if (j == n) l[n++] = {s, 1, 1, 0, 0};
+      (first ? l[j].na : l[j].nb) = r.count[i];
+    }
+  };
+  add(a, true);
+  add(b, false);
+  std::sort(l, l + n, [](const Level& p, const Level& q) { return p.stride < q.stride; });
+  long long ea = a.width * a.bytes, eb = b.width * b.bytes;
+  for (int i = 0; i < n; ++i) {
+    l[i].ea = ea;
+    l[i].eb = eb;
+    ea += (l[i].na - 1) * l[i].stride;
+    eb += (l[i].nb - 1) * l[i].stride;
+  }
+  return levels_apart(l, n, d, a.width * a.bytes, b.width * b.bytes);
 }
 
 namespace {
@@ -810,12 +848,14 @@ int launch_select(const EvictParams& p, int pairs, int device, cudaStream_t st) 
 bool pools_distinct(const SpinnCudaCache& c, int bytes) {
   const Rows k = {c.k, bytes, c.head_dim, {c.num_pages, c.page_size, c.kv_heads},
                   {c.page_stride, c.token_stride, c.head_stride}};
-  return rows_distinct(k) && c.k != c.v;
+  Rows v = k;
+  v.p = c.v;
+  return rows_distinct(k) && rows_apart(k, v);
 }
 
-bool overlap(const void* a, size_t na, const void* b, size_t nb) {
-  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-  return x < y + nb && y < x + na;
+// [rows][width] of 4-byte elements; one row: contiguous.
+Rows words(const void* p, long long width, long long rows = 1, long long stride = 0) {
+  return {p, 4, width, {rows, 1, 1}, {stride, 0, 0}};
 }
 
 }  // namespace
@@ -846,7 +886,7 @@ __attribute__((visibility("default"))) int spinn_cuda_stream_sync(void* stream) 
   }
   set_error("paged cache:%s%s%s", bits & kCacheBadPage ? " a page number outside the pool;" : "",
             bits & kCacheBadLength ? " a length outside its table, weights or rows;" : "",
-            bits & kCacheSamePage ? " an output page that the call reads (in place takes the same table pointer);" : "");
+            bits & kCacheSamePage ? " an output page that its row also reads (in place takes the same table pointer);" : "");
   return SPINN_CUDA_EINVAL;
 }
 
@@ -866,14 +906,14 @@ __attribute__((visibility("default"))) int spinn_cuda_cache_append(const SpinnCu
   const int es = dtype_bytes(cache->dtype);
   SPINN_CHECK_ARG(((uintptr_t)rows->k | (uintptr_t)rows->v) % es == 0 && (uintptr_t)rows->starts % 4 == 0,
                   "cache_append: misaligned pointer");
+  SPINN_CHECK_ARG(pools_distinct(*cache, es), "cache_append: the pools' rows overlap");
+  SPINN_CHECK_ARG(rows->tokens <= kMaxLength, "cache_append: %d tokens", rows->tokens);
   int dev;
   rc = check_stream_device("cache_append", stream, &dev);
   if (rc) return rc;
   if (rows->tokens == 0) return 0;
   rc = decode_error_word(dev, &p.c.err);
   if (rc) return rc;
-  SPINN_CHECK_ARG(pools_distinct(*cache, es), "cache_append: the pools' rows overlap");
-  SPINN_CHECK_ARG(rows->tokens <= kMaxLength, "cache_append: %d tokens", rows->tokens);
   p.k = rows->k;
   p.v = rows->v;
   p.k_tok = rows->k_token_stride;
@@ -920,23 +960,31 @@ __attribute__((visibility("default"))) int spinn_cuda_cache_evict(const SpinnCud
   SPINN_CHECK_ARG(!p.in_place || table->seqs == 1 || e->out_row_stride == table->row_stride,
                   "cache_evict: in place, the output table's stride must be the table's");
   p.same_weights = e->weights_in == e->weights_out;
-  const size_t wi = 4 * ((table->seqs - 1) * (size_t)e->win_seq_stride + (cache->kv_heads - 1) * (size_t)e->win_head_stride +
-                         e->weights_capacity);
-  const size_t wo = 4 * ((table->seqs - 1) * (size_t)e->wout_seq_stride +
-                         (cache->kv_heads - 1) * (size_t)e->wout_head_stride + e->weights_capacity);
+  const Rows weights = {e->weights_out, 4, e->weights_capacity, {table->seqs, cache->kv_heads, 1},
+                        {e->wout_seq_stride, e->wout_head_stride, 0}};
+  const Rows win = {e->weights_in, 4, e->weights_capacity, {table->seqs, cache->kv_heads, 1},
+                    {e->win_seq_stride, e->win_head_stride, 0}};
   SPINN_CHECK_ARG(p.same_weights ? e->win_seq_stride == e->wout_seq_stride && e->win_head_stride == e->wout_head_stride
-                                 : !overlap(e->weights_in, wi, e->weights_out, wo),
+                                 : rows_apart(weights, win),
                   "cache_evict: weights_out must be weights_in itself or apart from it");
+  const int es = dtype_bytes(cache->dtype);
+  SPINN_CHECK_ARG(pools_distinct(*cache, es), "cache_evict: the pools' rows overlap");
+  SPINN_CHECK_ARG(rows_distinct(weights), "cache_evict: rows of weights_out overlap");
+  // what is written against what is read and against one another
+  const Rows kept = words(e->kept, pairs * e->budget), new_lens = words(e->new_lens, table->seqs);
+  const Rows reads[] = {words(table->lens, table->seqs), words(table->pages, table->max_pages, table->seqs, table->row_stride),
+                        words(e->out_pages, e->out_max_pages, table->seqs, e->out_row_stride)};
+  for (const Rows& r : reads)
+    SPINN_CHECK_ARG(rows_apart(kept, r) && rows_apart(new_lens, r) && rows_apart(weights, r),
+                    "cache_evict: kept, new_lens or weights_out overlaps the lengths or a table");
+  SPINN_CHECK_ARG(rows_apart(kept, new_lens) && rows_apart(kept, weights) && rows_apart(new_lens, weights) &&
+                      rows_apart(kept, win) && rows_apart(new_lens, win),
+                  "cache_evict: kept, new_lens and the weights overlap one another");
   int dev;
   rc = check_stream_device("cache_evict", stream, &dev);
   if (rc) return rc;
   rc = decode_error_word(dev, &p.c.err);
   if (rc) return rc;
-  const int es = dtype_bytes(cache->dtype);
-  SPINN_CHECK_ARG(pools_distinct(*cache, es), "cache_evict: the pools' rows overlap");
-  const Rows weights = {e->weights_out, 4, e->weights_capacity, {table->seqs, cache->kv_heads, 1},
-                        {e->wout_seq_stride, e->wout_head_stride, 0}};
-  SPINN_CHECK_ARG(rows_distinct(weights), "cache_evict: rows of weights_out overlap");
   p.win = e->weights_in;
   p.wout = e->weights_out;
   p.win_seq = e->win_seq_stride;

@@ -80,8 +80,8 @@ struct Rows {
 // No two rows share an element (a tensor that is written must not: its rows are written by many
 // CTAs).  Dimensions nest, in any order.
 bool rows_distinct(const Rows& r);
-// No element of `a` is one of `b`.  Operands that interleave in one buffer (slices of its rows)
-// are told apart when their outermost strides agree.
+// No element of `a` is one of `b`.  Operands that interleave in one buffer (slices of its rows, keys and
+// values of one pool in any order of dimensions) are told apart where their strides agree.
 bool rows_apart(const Rows& a, const Rows& b);
 
 // The current device's deferred error word (device memory; DecodeErr bits).
