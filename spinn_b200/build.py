@@ -74,18 +74,22 @@ def _compile(src: str, force: bool, verbose: bool, extra: list) -> str:
     return obj
 
 
-def _build_torch_ops(force: bool, verbose: bool) -> str:
+def _build_torch_ops(force: bool, verbose: bool) -> None:
     """csrc/torch_ops.cpp against the installed torch; rebuilt when it, the C header or torch's
-    version changes."""
+    version changes.  Without torch there is nothing to bind: the C library is complete by itself."""
     import importlib.metadata
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        print("spinn_b200: torch is not installed, its binding (_torch_ops.so) is not built", file=sys.stderr)
+        return
     src = os.path.join(CSRC, "torch_ops.cpp")
     stamp = os.path.join(BUILD, "torch_ops.version")
     version = importlib.metadata.version("torch")
     newest = max(os.path.getmtime(src), _headers_mtime())
     if not force and os.path.exists(TORCH_OPS) and os.path.exists(stamp) and \
             os.path.getmtime(TORCH_OPS) >= newest and open(stamp).read() == version:
-        return TORCH_OPS
-    root = os.path.join(os.path.dirname(importlib.util.find_spec("torch").origin))
+        return
+    root = os.path.dirname(spec.origin)
     cxx = host_compiler()[-1] if host_compiler() else "g++"
     cmd = [cxx, "-O2", "-std=c++20", "-fPIC", "-shared", "-fvisibility=hidden", "-I" + os.path.join(root, "include"),
            "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
@@ -100,7 +104,6 @@ def _build_torch_ops(force: bool, verbose: bool) -> str:
         raise RuntimeError(f"{cxx} failed on torch_ops.cpp:\n{r.stdout}\n{r.stderr}")
     with open(stamp, "w") as f:
         f.write(version)
-    return TORCH_OPS
 
 
 def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = False) -> str:
