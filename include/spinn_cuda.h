@@ -172,7 +172,8 @@ int spinn_cuda_conv2d_noalloc(const float *x, const float *w, const float *bias,
 
 /* Waits for `stream` and returns (and clears) the deferred error of the operators below on the
  * current device: SPINN_CUDA_EINVAL for a bad page or length, SPINN_CUDA_ETIMEOUT for an
- * expired wait.  Refused while `stream` is being captured. */
+ * expired wait.  There is one error word per device: the first call on any stream reports what calls on
+ * all of them raised.  Refused while `stream` is being captured. */
 int spinn_cuda_stream_sync(void *stream);
 
 /* Two page pools of one shape: keys and values, [num_pages][page_size][kv_heads][head_dim] with
@@ -197,8 +198,9 @@ typedef struct {
 
 /* Appends new tokens: rows [starts[s], starts[s + 1]) of k and v ([tokens][kv_heads][head_dim],
  * strides in elements, the cache's type) become tokens lens[s], lens[s] + 1, ... of sequence s.
- * starts == NULL: one new token for each sequence (tokens == seqs).  lens is not changed.  Two
- * sequences may not write to the same page. */
+ * starts == NULL: one new token for each sequence (tokens == seqs).  Rows outside [starts[0],
+ * starts[seqs]) belong to no sequence: they are not written, and reported like a bad length.  lens is not
+ * changed.  Two sequences may not write to the same page. */
 typedef struct {
     const void *k, *v;
     int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
@@ -216,11 +218,16 @@ int spinn_cuda_cache_append(const SpinnCudaCache *cache, const SpinnCudaPageTabl
  * of length 0 gets zeros.  Sums are held in fp32 and y is rounded once; over 16-bit caches a probability
  * enters the product with v as two 16-bit parts, off by at most 2^-17 of itself (bf16) or of the largest
  * of 16 tokens around it (fp16).
- * weights_out, when not NULL ([seqs][kv_heads][>= lens[s]] fp32, group <= 16, weights_capacity
- * entries per row): weights_out[s][j][t] = weights_in[s][j][t] + the sum of p[s][h][t] over the
+ * weights_out, when not NULL ([seqs][kv_heads][>= lens[s]] fp32, group <= 16 over a 16-bit cache and <= 8
+ * over an fp32 one, weights_capacity entries per row): weights_out[s][j][t] = weights_in[s][j][t] + the sum of p[s][h][t] over the
  * heads h of group j, for t < lens[s]; entries beyond are left as they were.  weights_in NULL
- * counts as zeros; it may be weights_out itself, and may not overlap it otherwise.  Cached keys or
- * values that are not finite make the outputs that read them so. */
+ * counts as zeros; it may be weights_out itself, and may not overlap it otherwise.  The host does not
+ * know the lengths, so with weights the workspace holds the scores of the longest sequence that
+ * table and weights allow: 4 bytes per query head and token of seqs * min(max_pages * page_size,
+ * weights_capacity), 2.1 GB for 64 sequences of up to 131072 tokens and 64 query heads.  A smaller
+ * weights_capacity (at least the longest length) makes it smaller.  Cached keys or values that are not
+ * finite make the outputs that read them so.  Sequences times head blocks (a key head's queries in
+ * blocks of 8 or 16) times capacity / 32 may not pass 2^31 - 1. */
 typedef struct {
     const void *q;
     void *y;
@@ -246,7 +253,8 @@ int spinn_cuda_paged_attention(const SpinnCudaCache *cache, const SpinnCudaPageT
  * beyond are left as they were).  new_lens[s] = n.
  * out_pages == the table's pages (the same pointer): in place; then no page may belong to two
  * sequences, and out_row_stride is the table's.  Otherwise out_pages names pages that no
- * sequence of the call reads, no page twice, enough for n tokens per row.  weights_out may be weights_in. */
+ * sequence of the call reads, no page twice, enough for n tokens per row.  weights_out may be weights_in.
+ * seqs * kv_heads is at most 65535. */
 typedef struct {
     const float *weights_in;
     float *weights_out;
@@ -264,7 +272,7 @@ int spinn_cuda_cache_evict(const SpinnCudaCache *cache, const SpinnCudaPageTable
 
 /* Linear layer: y = act(x w^T + bias) + residual, x [m][k], w [n][k], y and residual [m][n], bias
  * [n], all of one 16-bit type (dtype SPINN_CUDA_FP16 or _BF16; the fp32 form is
- * spinn_cuda_gemm).  Rows are contiguous, row strides in elements.  Products accumulate in fp32
+ * spinn_cuda_gemm).  Rows are contiguous, row strides in elements and at least a row's length.  Products accumulate in fp32
  * and y is rounded once.  bias and residual may be NULL; y may be the residual itself.
  * act: the ENNF fused-act codes 0 (none), 1 (ReLU), 3 (SiLU), and 6 (GELU, by erf), 7 (GELU, by
  * tanh); unlike the convolutions' 4 and 5 the residual is added after the activation. */

@@ -66,14 +66,14 @@ __device__ __forceinline__ T round_to(float x) {
 // The activations of the fp32 accumulators, chosen once per block of values: a switch per value
 // cost a third of a whole launch (4096 x 4096 x 8192 with SiLU: 234 us, 207 us without it).  SiLU
 // and the tanh form share v / (1 + e^-z): the tanh form is 0.5 v (1 + tanh u) = v / (1 + e^(-2 u)).
-// The fast exponential and quotient are off by a few ulp of fp32, far below the rounding of y.
+// The fast quotient is off by 2 ulp of fp32, the fast exponential by 2 + 1.17 |z| (some 100 where it leaves
+// fp32's range, 2^-16): far below the rounding of y.
 //
 // GELU by erf: v Phi(v) with Phi(-|v|) = erfc(x) / 2, x = |v| / sqrt(2), and erfc(x) = t e^(Q(t) - x^2),
 // t = 1 / (1 + 0.6 x).  Q is a degree-8 Chebyshev fit over t in (0, 1] of the logarithm of the scaled
 // function, erfc(x) e^(x^2) / t, in powers of two and with the factor 1/2 in its constant: within
-// 5e-6 of the value everywhere in fp32, the tail included (checked over [-9, 9]), in a third of
-// erff's instructions (777 x 1024 x 2048
-// 10.5 us, 11.5 with erff).
+// 5e-6 of the value over [-9, 9] and 1e-5 down to -13, where the value leaves fp32's normal range and becomes
+// 0, in a third of erff's instructions (777 x 1024 x 2048 10.5 us, 11.5 with erff).
 __device__ __forceinline__ float gelu_erf(float v) {
   const float t = __fdividef(1.0f, fmaf(0.42426407f, fabsf(v), 1.0f));  // 0.6 / sqrt(2)
   float q = 0.268522114f;

@@ -139,7 +139,8 @@ def _ops():
 
 def stream_sync(device: Optional[int] = None) -> None:
     """Waits for torch's current stream and raises the deferred error of the operators below, if
-    any (``spinn_cuda_stream_sync``).  Not during graph capture."""
+    any (``spinn_cuda_stream_sync``): of calls on every stream of the device, which share one error word.
+    Not during graph capture."""
     import torch
     with torch.cuda.device(device):
         check(lib().spinn_cuda_stream_sync(torch.cuda.current_stream().cuda_stream), "spinn_cuda_stream_sync")
@@ -149,8 +150,8 @@ def linear(x, w, y, bias=None, residual=None, act: str = "none") -> None:
     """``y = act(x @ w.T + bias) + residual`` in fp16 or bf16 (fp32: :func:`gemm`), accumulated in fp32
     and rounded once.
 
-    ``x`` is ``[m, k]``, ``w`` ``[n, k]``, ``y`` and ``residual`` ``[m, n]``, with contiguous rows of any
-    stride, ``bias`` ``[n]``; ``act`` is "none", "relu", "silu", "gelu" (by erf) or "gelu_tanh".  ``y``
+    ``x`` is ``[m, k]``, ``w`` ``[n, k]``, ``y`` and ``residual`` ``[m, n]``, with contiguous rows a row's
+    length or more apart (no expanded rows), ``bias`` ``[n]``; ``act`` is "none", "relu", "silu", "gelu" (by erf) or "gelu_tanh".  ``y``
     may be ``residual`` itself.  Rows of ``x`` and ``w`` that start on 16-byte boundaries are read in
     place; others are copied first where tiles serve better than the kernel for few rows."""
     code = _ACTS.get(act)
@@ -163,7 +164,8 @@ def cache_append(k, v, k_cache, v_cache, page_table, lens, starts=None) -> None:
     """Writes new tokens' rows ``k`` and ``v`` ``[tokens, kv_heads, head_dim]`` into the paged cache.
 
     Rows ``starts[s] .. starts[s + 1] - 1`` (int32, ``[seqs + 1]``) become tokens ``lens[s]``,
-    ``lens[s] + 1``, ... of sequence ``s``; without ``starts`` there is one row per sequence.
+    ``lens[s] + 1``, ... of sequence ``s``; without ``starts`` there is one row per sequence.  Rows outside
+    ``starts[0] .. starts[-1]`` are not written, and reported by :func:`stream_sync`.
     ``lens`` (the lengths before) is not changed.  Caches are ``[pages, page_size, kv_heads,
     head_dim]`` in fp32, fp16 or bf16 with any strides but a contiguous last dimension,
     ``page_table`` is int32 ``[seqs, max_pages]``."""
@@ -177,7 +179,10 @@ def paged_attention(q, k_cache, v_cache, page_table, lens, y, scale=None, weight
     ``h // (q_heads // kv_heads)``.  ``scale`` defaults to ``head_dim ** -0.5``.  A sequence of
     length 0 gets zeros.  With ``weights_out`` (fp32 ``[seqs, kv_heads, length]``) the probabilities
     of each key head's queries are summed and added to ``weights`` (zeros when None; may be
-    ``weights_out`` itself); entries past a sequence's length are left as they were."""
+    ``weights_out`` itself); entries past a sequence's length are left as they were.  That takes at most
+    16 queries to a key head (8 over an fp32 cache), and a workspace of 4 bytes per query head and token
+    that table and weights have room for: views of the weights no longer than the longest cache keep
+    it small."""
     (_binding or _ops()).paged_attention(q, k_cache, v_cache, page_table, lens, y, scale, weights, weights_out)
 
 
