@@ -819,17 +819,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
 // Four warps of a group wait for a barrier that a fifth completes after `arrive_ns`; the first gives up
 // after `limit_ns`, by an abort flag of its own.  Bit w of the result: warp w goes on.
-__device__ unsigned g_group_wait_verdict;
+__device__ unsigned g_group_went_on;
 __global__ void __launch_bounds__(160) group_wait_selftest_kernel(uint64_t arrive_ns, uint64_t limit_ns) {
   __shared__ uint64_t bar;
   __shared__ int abort_flag[2];
-  __shared__ unsigned verdict;
+  __shared__ unsigned went_on;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(&bar, 1);
     fence_mbar_init();
     abort_flag[0] = abort_flag[1] = 0;
-    verdict = 0;
+    went_on = 0;
   }
   __syncthreads();
   if (warp == 4) {
@@ -840,10 +840,10 @@ __global__ void __launch_bounds__(160) group_wait_selftest_kernel(uint64_t arriv
     }
   } else {
     const bool on = group_wait(&bar, 0, &abort_flag[warp != 0], warp ? kTimeoutNs : limit_ns, 0);
-    if (on && lane == 0) atomicOr(&verdict, 1u << warp);
+    if (on && lane == 0) atomicOr(&went_on, 1u << warp);
   }
   __syncthreads();
-  if (threadIdx.x == 0) g_group_wait_verdict = verdict;
+  if (threadIdx.x == 0) g_group_went_on = went_on;
 }
 
 // ------------------------------------------------------------------ host
@@ -1062,9 +1062,9 @@ __attribute__((visibility("default"))) int spinn_cuda_selftest_group_wait(uint64
                   "selftest_group_wait: at most 100 ms to the arrival and a limit of at most 1 s");
   group_wait_selftest_kernel<<<1, 160>>>(arrive_ns, limit_ns);
   SPINN_CUDA_TRY(cudaGetLastError());
-  unsigned verdict = 0;
-  SPINN_CUDA_TRY(cudaMemcpyFromSymbol(&verdict, g_group_wait_verdict, sizeof(verdict)));
-  return (int)verdict;
+  unsigned went_on = 0;
+  SPINN_CUDA_TRY(cudaMemcpyFromSymbol(&went_on, g_group_went_on, sizeof(went_on)));
+  return (int)went_on;
 }
 
 __attribute__((visibility("default"))) int spinn_cuda_diag_linear_plan(const SpinnCudaLinear* l, int sms, int* out5) {
